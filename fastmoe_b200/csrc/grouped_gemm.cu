@@ -17,9 +17,7 @@
 //               while the next tile's MMAs fill the other accumulator
 // Every mbarrier wait is bounded: on a timeout the kernel sets FMOE_STATUS_WAIT_TIMEOUT in
 // the status word, every role leaves its loop, TMEM is released and the kernel returns.
-#include <cuda.h>
-
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace fmoe {
 
@@ -56,134 +54,9 @@ struct GemmArgs {
   int32_t* status;
 };
 
-// ---- PTX wrappers -------------------------------------------------------------------
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
-               : "memory");
-}
-// Bounded wait: false after `limit` unsuccessful probes, or once another role has given up.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                          uint32_t limit) {
-  const uint32_t addr = smem_u32(bar);
-  for (uint32_t spin = 0; spin < limit; ++spin) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(addr), "r"(parity)
-        : "memory");
-    if (done) return true;
-    if ((spin & 1023u) == 1023u && *abort_flag) return false;
-  }
-  return false;
-}
-// The same without the give-up flag: used on the way out, when the flag may already be set.
-__device__ __forceinline__ bool mbar_wait_plain(uint64_t* bar, uint32_t parity, uint32_t limit) {
-  int never = 0;
-  return mbar_wait(bar, parity, &never, limit);
-}
-// Leaving the kernel, normally or after a wait gave up: the MMA thread waits (bounded) until
-// the tensor core has finished every MMA it issued, so that tensor memory is not released
-// under them; after a give-up the producer thread waits (bounded) for the loads it still has
-// in flight, so that none lands in shared memory after the CTA has gone.
-__device__ __forceinline__ void drain_on_exit(int warp, int lane, int fills, bool mma_issued, uint64_t* full,
-                                              uint64_t* drain, const volatile int* abort_flag, int stages,
-                                              uint32_t limit) {
-  if (warp == 0 && lane == 0 && *abort_flag) {
-    for (int s = 0; s < stages && s < fills; ++s) {
-      const int last = (fills - 1 - s) / stages * stages + s;  // last fill that used stage s
-      mbar_wait_plain(&full[s], (last / stages) & 1, limit);
-    }
-  }
-  if (warp == 1 && lane == 0 && mma_issued) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                     static_cast<uint32_t>(__cvta_generic_to_shared(drain)))
-                 : "memory");
-    mbar_wait_plain(drain, 0, limit);
-  }
-}
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
-      : "memory");
-}
-__device__ __forceinline__ void tcgen05_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tcgen05_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
-                                          uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// Arrives on `bar` once every MMA issued so far by this thread has completed.
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// Shared-memory operand descriptor: K-major tile, 128-byte swizzle, rows 128 bytes apart,
-// 8-row groups 1024 bytes apart (the layout a 128B-swizzled TMA box produces).
-__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((saddr >> 4) & 0x3fff);        // start address
-  d |= static_cast<uint64_t>(1) << 16;                       // leading byte offset (unused here)
-  d |= static_cast<uint64_t>((1024 >> 4) & 0x3fff) << 32;    // stride byte offset
-  d |= static_cast<uint64_t>(1) << 46;                       // descriptor version (sm_100)
-  d |= static_cast<uint64_t>(2) << 61;                       // 128-byte swizzle
-  return d;
-}
-// The same for an operand whose MN dimension is the contiguous one (a row-major [K, N] weight
-// used as B): 64-element (128-byte) pieces of the MN dimension are separate TMA boxes
-// `mn_piece_bytes` apart, and inside a box every 8 reduction rows form a 1024-byte group.
-__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr, uint32_t mn_piece_bytes) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((saddr >> 4) & 0x3fff);
-  d |= static_cast<uint64_t>((mn_piece_bytes >> 4) & 0x3fff) << 16;  // leading byte offset: next MN piece
-  d |= static_cast<uint64_t>((1024 >> 4) & 0x3fff) << 32;            // stride byte offset: next 8 reduction rows
-  d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(2) << 61;
-  return d;
-}
 // Instruction descriptor: D fp32, A and B bf16, both K-major, M=128, N=256.
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kBN >> 3) << 17) | ((kBM >> 4) << 24);
 constexpr uint32_t kIdescBMn = kIdesc | (1u << 16);  // B with the N dimension contiguous
-
-__device__ __forceinline__ float silu(float x) { return x / (1.f + __expf(-x)); }
-__device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.f + erff(x * 0.70710678118654752f)); }
-
-// Rows of expert e that lie inside A: a count that would run past the end of A (a caller
-// whose receive buffer overflowed, say) is cut there, so no tile reaches beyond row R.
-__device__ __forceinline__ int64_t expert_rows(const int64_t* offsets, const int64_t* counts, int64_t R, int e) {
-  const int64_t off = offsets[e], n = counts[e];
-  if (off < 0 || off >= R || n <= 0) return 0;
-  return n < R - off ? n : R - off;
-}
 
 // Asks for a tile to be brought into L2; completes on its own, nothing waits for it.
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int c0, int c1) {
@@ -1041,28 +914,10 @@ int g_gemm_spin_limit = static_cast<int>(kSpinLimit);
 int g_gemm_tokens_as_n = -1;
 constexpr int64_t kTnAutoRows = 0;  // rows per expert below which "auto" picks tokens-as-N (0: never)
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_tiled_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (fn == nullptr) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  }
-  return fn;
-}
-
 // 2-D bf16 row-major tensor [rows, cols], box = 64 columns x box_rows rows, 128-byte swizzle.
 static int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, const char* what,
                     int box_rows = 128) {
-  // The encoder is a driver call and wants a current context. A thread that has not yet made
-  // a runtime call of this library (an autograd worker, say) may have none bound: bind it.
-  FMOE_CUDA(cudaFree(nullptr));
+  if (const int rc = bind_context(); rc != 0) return rc;
   EncodeTiledFn fn = encode_tiled_fn();
   FMOE_REQUIRE(fn != nullptr, FMOE_ERR_DEVICE, "fmoe_grouped_gemm: cuTensorMapEncodeTiled is not available");
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
