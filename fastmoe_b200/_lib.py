@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import c_char_p, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_double, c_int, c_int64, c_size_t, c_void_p
 
 from . import build as _build
 
@@ -56,6 +56,15 @@ SIGNATURES = {
     "fmoe_permute_peer_fwd": (c_int, [_P, _L, _P, _P, _P, _P, _P, _L, _L, _L, _L, _L, _L, _P, _L, _L, _I, _P, _P]),
     "fmoe_peer_barrier": (c_int, [_P, _L, _L, ctypes.c_int32, _L, _P, _P]),
     "fmoe_ep_layout": (c_int, [_P, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "fmoe_rms_norm": (c_int, [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _L, _P, _L, _L, c_double, _I, _P]),
+    "fmoe_rms_norm_bwd_bytes": (c_size_t, [_L, _L]),
+    "fmoe_rms_norm_bwd": (c_int, [_P, _L, _P, _L, _P, _L, _P, _P, _I, _P, _P, _P, c_size_t, _L, _L, _I, _P]),
+    "fmoe_quantize_rows": (c_int, [_P, _L, _P, _L, _P, _L, _L, _I, _P]),
+    "fmoe_dequantize_rows": (c_int, [_P, _L, _P, _P, _L, _L, _I, _P]),
+    "fmoe_int8_gemm": (c_int, [_P, _L, _P, _P, _L, _L, _P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _P, _P]),
+    "fmoe_pack_activation": (c_int, [_P, _L, _P, _L, _P, _L, _L, _I, _P]),
+    "fmoe_unpack_activation": (c_int, [_P, _L, _P, _P, _L, _L, _I, _P]),
+    "fmoe_packed_act_bwd": (c_int, [_P, _L, _P, _P, _L, _P, _P, _L, _L, _I, _I, _P]),
     "fmoe_combine_host_arena_bytes": (c_size_t, [_P, _L, _L, _L, _L, _I]),
     "fmoe_combine_host": (c_int, [_P, _P, _P, _I, _P, _I, _P, _L, _L, _L, _L, _I, _P, c_size_t, _P]),
 }

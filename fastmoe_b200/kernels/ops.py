@@ -300,6 +300,15 @@ def _call(fn_name, n_kernels, *args):
     return rc
 
 
+def _launch(device, fn_name, n_kernels, *args):
+    """`_call` on `device`'s current stream (appended as the last argument), with that device made
+    current for the launch where it is not."""
+    if device.index == torch.cuda.current_device():
+        return _call(fn_name, n_kernels, *args, _stream_ptr(device))
+    with torch.cuda.device(device):
+        return _call(fn_name, n_kernels, *args, _stream_ptr(device))
+
+
 def _combine_into(expert_tensors, indices, weights, out, metadata, accumulate, mode=None):
     """Runs the combine into `out` ([T, D], any row stride). Returns the plan (or None)."""
     mode = _mode if mode is None else mode

@@ -406,6 +406,74 @@ int fmoe_swiglu_bwd_ragged(const void* h, const void* grad_act, void* grad_h, in
 int fmoe_gelu_bwd(const void* h, const void* grad_act, void* grad_h, int64_t rows, int64_t n,
                   void* stream);
 
+/* ---- RMS norm and 8-bit rows -------------------------------------------------- */
+/*
+ * The norm of the residual stream that a block's attention and feed-forward read:
+ *   s = x + residual, rounded to the rows' type      (without a residual: s = x)
+ *   rstd = 1 / sqrt(mean(s^2) + eps)                 y = s * rstd * w
+ * and, for a consumer that multiplies in 8 bits (fmoe_int8_gemm), the row in 8 bits:
+ *   a = max(largest |y| of the row, 2^-100), q = round(y * 127 / a) (ties to even), q_scale = a / 127
+ * y is quantised from its fp32 value, before the rounding to the rows' type. A row that holds
+ * NaN or infinity gets q = 0 and q_scale = NaN, so that all that is computed from it reads NaN.
+ * x, residual [T, D] with row strides in elements; w [D] (fp32 or the rows' type); y, sum [T, D]
+ * contiguous; rstd optional float[T] for the backward pass; q int8 [T, D] with a row stride that
+ * is a multiple of 16 (the bytes from D up to the next multiple of 16 are zeroed). y or q may be
+ * NULL; sum receives s and goes with residual. The reference's blocks normalise with LayerNorm
+ * (src/fastmoe/models/tiny_model.py:424-463).
+ */
+int fmoe_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t r_stride, const void* w,
+                  int w_dtype, void* y, void* sum, float* rstd, int8_t* q, int64_t q_stride, float* q_scale,
+                  int64_t T, int64_t D, double eps, int dtype, void* stream);
+
+/* Gradient: with xh = sum * rstd and g = dy * w, dx = rstd * (g - xh * mean(g * xh)) + dsum (dsum:
+ * the gradient that reaches s itself, optional) and dw = sum over rows of dy * xh (optional, in
+ * w's type). dx is the gradient of x and of the residual alike. dw is added up in a fixed order.
+ * scratch: fmoe_rms_norm_bwd_bytes(T, D) bytes, needed with dw. */
+size_t fmoe_rms_norm_bwd_bytes(int64_t T, int64_t D);
+int fmoe_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dsum, int64_t ds_stride, const void* sum,
+                      int64_t s_stride, const float* rstd, const void* w, int w_dtype, void* dx, void* dw,
+                      void* scratch, size_t scratch_bytes, int64_t T, int64_t D, int dtype, void* stream);
+
+/* Rows of x in 8 bits, one scale per row (the convention above), and back: out = q * q_scale. */
+int fmoe_quantize_rows(const void* x, int64_t x_stride, int8_t* q, int64_t q_stride, float* q_scale, int64_t T,
+                       int64_t D, int dtype, void* stream);
+int fmoe_dequantize_rows(const int8_t* q, int64_t q_stride, const float* q_scale, void* out, int64_t T, int64_t D,
+                         int dtype, void* stream);
+
+/* ---- matrix product in 8-bit integers ------------------------------------------- */
+/*
+ * C[r, n] = act((sum_k a[r, k] * w[e, n, k]) * a_scale[r] * w_scale[e, n]) for the rows r of expert e,
+ * rows [offsets[e], offsets[e] + counts[e]) as in fmoe_grouped_gemm; offsets = counts = NULL and
+ * E = 1: one dense product. The sum is exact in 32-bit integers; scales and activation in fp32; one
+ * rounding to out_dtype. a int8 [R, K], w int8 [E, N, K]: row strides (and w's expert stride) in
+ * bytes, multiples of 16, at least K; any R, N and K < 131072 (the bytes from K up to the next
+ * multiple of 16 must be readable; what they hold does not matter). C contiguous, [R, N], or [R, N/2] for
+ * FMOE_ACT_SWIGLU (gate rows of w first). Rows outside every expert are not touched. E <= 1024. An
+ * expert whose range runs past row R is cut off there (FMOE_STATUS_BAD_EXPERT).
+ */
+int fmoe_int8_gemm(const int8_t* a, int64_t a_stride, const float* a_scale, const int8_t* w, int64_t w_stride,
+                   int64_t w_expert_stride, const float* w_scale, void* c, const int64_t* offsets,
+                   const int64_t* counts, int64_t E, int64_t R, int64_t N, int64_t K, int activation,
+                   int out_dtype, int32_t* status, void* stream);
+
+/* ---- activations kept in 8 bits for the backward pass ---------------------------- */
+/*
+ * pack: each group of 128 columns of a row (the last one may be shorter) as int8 values and one fp32
+ * scale, by the convention of fmoe_rms_norm's 8-bit rows; q [T, D] with row stride D rounded up to
+ * 16 bytes (zeros in between), scale float[T, ceil(D / 128)]. unpack: out = q * scale.
+ * fmoe_packed_act_bwd: the derivative of an expert's activation from its packed pre-activations h~:
+ *   FMOE_ACT_SWIGLU  h~ = [gate | up], D = 2*ff: grad_h = [d_gate | d_up], hidden = silu(gate) * up
+ *   FMOE_ACT_GELU    grad_h = grad * gelu'(h~), hidden = gelu(h~)
+ * grad, hidden [T, ff] (or [T, D]); hidden is what the second product's weight gradient needs, so a
+ * forward pass that packs its pre-activations keeps neither them nor hidden in 16 bits.
+ */
+int fmoe_pack_activation(const void* x, int64_t x_stride, int8_t* q, int64_t q_stride, float* scale, int64_t T,
+                         int64_t D, int dtype, void* stream);
+int fmoe_unpack_activation(const int8_t* q, int64_t q_stride, const float* scale, void* out, int64_t T,
+                           int64_t D, int dtype, void* stream);
+int fmoe_packed_act_bwd(const int8_t* q, int64_t q_stride, const float* scale, const void* grad, int64_t g_stride,
+                        void* grad_h, void* hidden, int64_t T, int64_t D, int activation, int dtype, void* stream);
+
 /* ---- host-buffer call -------------------------------------------------------- */
 /*
  * The whole combine for a caller that holds HOST memory: copies the E expert
