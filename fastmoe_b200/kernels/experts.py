@@ -17,9 +17,10 @@ alike: there is no library fallback.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from . import ops
+from . import checkpoint, ops
 from .ops import _require_cuda, _status_word, _stream_ptr
 
 ACT_NONE, ACT_SWIGLU, ACT_GELU = _lib.ACT_NONE, _lib.ACT_SWIGLU, _lib.ACT_GELU
@@ -202,16 +203,80 @@ def grouped_gemm(a, w, offsets, counts, swiglu=False, row_map=None, covers_all_r
     return _apply(a, w, offsets, counts, act, row_map, bool(covers_all_rows))
 
 
-def grouped_swiglu_ffn(x, w_gate_up, w_down, offsets, counts, row_map=None, covers_all_rows=False):
+class _PackedFFN(torch.autograd.Function):
+    """Both products of an expert with what the backward pass needs kept in 8 bits: the rows (for the
+    first weight's gradient) and the pre-activations; the hidden rows are recomputed from those."""
+
+    @staticmethod
+    def forward(ctx, x, w1, w2, offsets, counts, act, row_map, covers_all_rows):
+        pre = torch.empty(x.shape[0], w1.shape[1], dtype=torch.bfloat16, device=x.device)
+        hidden = _launch(x, w1, offsets, counts, act, covers_all_rows=covers_all_rows, pre=pre)
+        out = _launch(hidden, w2, offsets, counts, ACT_NONE, row_map, covers_all_rows)
+        p = checkpoint.pack_activation(pre)
+        px = checkpoint.pack_activation(x) if ctx.needs_input_grad[1] else None
+        ctx.save_for_backward(p.q, p.scale, None if px is None else px.q, None if px is None else px.scale, w1, w2,
+                              offsets, counts, row_map)  # fmt: skip
+        ctx.shapes = (p.shape, x.shape)
+        ctx.act, ctx.covers_all_rows = act, covers_all_rows
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        q, scale, xq, xscale, w1, w2, offsets, counts, row_map = ctx.saved_tensors
+        pre_shape, x_shape = ctx.shapes
+        if row_map is not None:
+            grad_out = grad_out.index_select(0, row_map)  # back to the row order of `x`
+        grad_out = grad_out.contiguous()
+        grad_hidden = _dgrad(grad_out, w2, offsets, counts, ctx.covers_all_rows)
+        packed = checkpoint.PackedActivation(q, scale, pre_shape, torch.bfloat16)
+        derivative = checkpoint.packed_swiglu_backward if ctx.act == ACT_SWIGLU else checkpoint.packed_gelu_backward
+        grad_pre, hidden = derivative(packed, grad_hidden)
+        del grad_hidden
+        grad_x = grad_w1 = grad_w2 = None
+        if ctx.needs_input_grad[2]:
+            grad_w2 = _wgrad(grad_out, hidden, w2.shape, offsets, counts)
+        del hidden
+        if ctx.needs_input_grad[1]:
+            x = checkpoint.unpack_activation(checkpoint.PackedActivation(xq, xscale, x_shape, torch.bfloat16))
+            grad_w1 = _wgrad(grad_pre, x, w1.shape, offsets, counts)
+        if ctx.needs_input_grad[0]:
+            grad_x = _dgrad(grad_pre, w1, offsets, counts, ctx.covers_all_rows)
+        return grad_x, grad_w1, grad_w2, None, None, None, None, None
+
+
+def _packed_ffn(x, w1, w2, offsets, counts, act, row_map, covers_all_rows):
+    _check(x, w1, offsets, counts)
+    ff = w1.shape[1] // 2 if act == ACT_SWIGLU else w1.shape[1]
+    if w2.dim() != 3 or w2.dtype != torch.bfloat16 or w2.shape[0] != w1.shape[0] or w2.shape[2] != ff:
+        raise ValueError(f"the second weight must be bfloat16 [{w1.shape[0]}, N, {ff}], got {tuple(w2.shape)} {w2.dtype}")
+    if row_map is not None and (row_map.dtype != torch.int64 or row_map.numel() != x.shape[0]):
+        raise ValueError("row_map must be an int64 device tensor with one entry per row of x")
+    check_shapes(w1.shape[1], w1.shape[2], act, True)
+    check_shapes(w2.shape[1], w2.shape[2], ACT_NONE, True)
+    return _PackedFFN.apply(x.contiguous(), w1, w2, offsets, counts, act, row_map, covers_all_rows)
+
+
+def _training(*tensors):
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+def grouped_swiglu_ffn(x, w_gate_up, w_down, offsets, counts, row_map=None, covers_all_rows=False, packed=False):
     """down(silu(gate(x)) * up(x)) per expert. w_gate_up [E, 2*ff, D] (gate rows first), w_down [E, D, ff].
-    `row_map` reorders the rows of the result (see grouped_gemm)."""
+    `row_map` reorders the rows of the result (see grouped_gemm). `packed=True`: a forward that will
+    be differentiated keeps the rows and the pre-activations in 8 bits and no hidden rows
+    (`kernels/checkpoint.py`): the result is the same, the gradients are taken at the kept values."""
+    if packed and _training(x, w_gate_up, w_down):
+        return _packed_ffn(x, w_gate_up, w_down, offsets, counts, ACT_SWIGLU, row_map, bool(covers_all_rows))
     hidden = grouped_gemm(x, w_gate_up, offsets, counts, activation=ACT_SWIGLU, covers_all_rows=covers_all_rows)
     return grouped_gemm(hidden, w_down, offsets, counts, row_map=row_map, covers_all_rows=covers_all_rows)
 
 
-def grouped_gelu_ffn(x, w1, w2, offsets, counts, row_map=None, covers_all_rows=False):
+def grouped_gelu_ffn(x, w1, w2, offsets, counts, row_map=None, covers_all_rows=False, packed=False):
     """fc2(gelu(fc1(x))) per expert, bias-free: the reference's expert (tiny_model.py:68-77).
-    w1 [E, ff, D], w2 [E, D, ff], both in nn.Linear layout."""
+    w1 [E, ff, D], w2 [E, D, ff], both in nn.Linear layout. `packed` as in grouped_swiglu_ffn."""
+    if packed and _training(x, w1, w2):
+        return _packed_ffn(x, w1, w2, offsets, counts, ACT_GELU, row_map, bool(covers_all_rows))
     hidden = grouped_gemm(x, w1, offsets, counts, activation=ACT_GELU, covers_all_rows=covers_all_rows)
     return grouped_gemm(hidden, w2, offsets, counts, row_map=row_map, covers_all_rows=covers_all_rows)
 

@@ -7,6 +7,7 @@ of `MoEFeedForward.gate_and_sort` in polkadot21/fastmoe
   route_topk        torch.topk + softmax(dtype=fp32).type_as(x)        (:97-100)
   build_index       argsort + gathers + bincount + per-rank sums       (:105-153)
   permute_rows      x_flat[reverse_map]                                (:133)
+                    (permute_int8_rows: the same for rows in 8 bits)
 
 The sorted order is the stable one (expert id, then flat routed position t*K+k);
 the reference's own order inside an expert segment is whatever an unstable
@@ -21,6 +22,7 @@ import torch
 
 from .. import _lib
 from . import ops
+from .int8 import Int8Rows, _operand, _padded
 from .ops import _DTYPES, _require_cuda, _status_word, _stream_ptr
 
 
@@ -156,3 +158,13 @@ def permute_rows(x: torch.Tensor, slot_of: torch.Tensor, K: int) -> torch.Tensor
     """permuted[slot_of[t*K+k]] = x[t]: the dispatch permute, each token row read once.
     Backward sums the K routed gradient rows of a token in fp32."""
     return _PermuteRows.apply(x, slot_of, int(K))
+
+
+def permute_int8_rows(rows: Int8Rows, ix: RoutingIndex, K: int) -> Int8Rows:
+    """The dispatch permute for rows in 8 bits: a token's bytes and scale at every sorted slot of it."""
+    q = _operand(rows.q)
+    T, D = q.shape
+    if D % 16:  # the rows travel with their padding, as 16-bit words
+        q = q.as_strided((T, _padded(D)), (q.stride(0), 1))
+    words = permute_rows(q.view(torch.bfloat16), ix.slot_of, K)
+    return Int8Rows(words.view(torch.int8)[:, :D], rows.scale[ix.reverse_map])

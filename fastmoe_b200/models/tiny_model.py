@@ -19,6 +19,11 @@ unpermute, tiny_model.py:42-420). What differs, on purpose:
     launches (activation fused in the first one's epilogue) instead of a Python loop of
     per-expert library calls.
 
+Beyond the reference's models, every block takes `norm="rms"` (RMS norm fused with the residual sum
+instead of LayerNorm) and `pack_activations=True` (training keeps the experts' activations in 8 bits),
+and `quantize_int8()` on a model, a block or a layer turns its products to 8-bit integers for
+inference.
+
 There is no CPU path: inputs must live on a CUDA device.
 """
 
@@ -32,9 +37,65 @@ from torch.profiler import record_function
 
 from .. import consts, exchange
 from ..kernels import experts as expert_kernels
-from ..kernels import routing
+from ..kernels import int8, routing
+from ..kernels import norm as norm_kernels
 from ..kernels.experts import grouped_gelu_ffn, grouped_swiglu_ffn
 from ..kernels.ops import grouped_weighted_scatter_add, routed_combine
+
+
+class RMSNorm(nn.Module):
+    """x / sqrt(mean(x^2) + eps) * weight over the last dimension (kernels/norm.py). Called with a
+    residual it returns (the norm of x + residual, x + residual)."""
+
+    def __init__(self, dim, eps=1e-6):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(dim))
+
+    @staticmethod
+    def _same_type(x, residual):
+        if residual is None or x.dtype == residual.dtype:
+            return x, residual
+        dtype = torch.promote_types(x.dtype, residual.dtype)  # under autocast: a bf16 branch beside an fp32 stream
+        return x.to(dtype), residual.to(dtype)
+
+    def forward(self, x, residual=None):
+        if residual is None:
+            return norm_kernels.rms_norm(x, self.weight, self.eps)
+        return norm_kernels.add_rms_norm(*self._same_type(x, residual), self.weight, self.eps)
+
+    def int8(self, x, residual=None, with_y=False):
+        """The normed rows in 8 bits (`norm_kernels.NormInt8`), for inference."""
+        x, residual = self._same_type(x, residual)
+        return norm_kernels.rms_norm_int8(x, self.weight, self.eps, residual=residual, with_y=with_y)
+
+
+def _make_norm(kind, dim):
+    if kind == "layer":
+        return nn.LayerNorm(dim)
+    if kind == "rms":
+        return RMSNorm(dim)
+    raise ValueError(f"norm must be 'layer' or 'rms', got {kind!r}")
+
+
+class Int8Linear(nn.Module):
+    """A bias-free nn.Linear for inference: weights in 8 bits with a scale per output channel, inputs
+    quantised row by row. Calling it with `rows` (the 8-bit form of x, from a norm) skips that; x then
+    only gives the shape and type of the result."""
+
+    def __init__(self, linear):
+        super().__init__()
+        if linear.bias is not None:
+            raise ValueError("Int8Linear takes a linear without bias")
+        q, scale = int8.quantize_weight(linear.weight)
+        self.register_buffer("weight_q", q)
+        self.register_buffer("weight_scale", scale)
+
+    def forward(self, x, rows=None):
+        if rows is None:
+            rows = int8.quantize_rows(x)
+        out = int8.int8_linear(rows, int8.Int8Weight(self.weight_q, self.weight_scale), out_dtype=x.dtype)
+        return out.view(*x.shape[:-1], out.shape[-1])
 
 
 class MultiheadSelfAttention(nn.Module):
@@ -48,9 +109,20 @@ class MultiheadSelfAttention(nn.Module):
         self.qkv = nn.Linear(dim, 3 * dim, bias=False)
         self.proj = nn.Linear(dim, dim, bias=False)
 
-    def forward(self, x):
+    @property
+    def is_int8(self):
+        return isinstance(self.qkv, Int8Linear)
+
+    def quantize_int8(self):
+        """Both projections in 8 bits, for inference."""
+        if not self.is_int8:
+            self.qkv, self.proj = Int8Linear(self.qkv), Int8Linear(self.proj)
+        return self
+
+    def forward(self, x, rows=None):
         B, T, D = x.shape
-        q, k, v = self.qkv(x).view(B, T, 3, self.n_heads, self.hd).permute(2, 0, 3, 1, 4)
+        qkv = self.qkv(x) if rows is None else self.qkv(x, rows)
+        q, k, v = qkv.view(B, T, 3, self.n_heads, self.hd).permute(2, 0, 3, 1, 4)
         y = F.scaled_dot_product_attention(q, k, v, is_causal=False)
         return self.proj(y.transpose(1, 2).reshape(B, T, D))
 
@@ -99,17 +171,22 @@ class GroupedSwiGLUExperts(nn.Module):
     def __iter__(self):
         return (self.expert(e) for e in range(self.num_experts))
 
-    def forward(self, x, offsets, counts, row_map=None):
+    def forward(self, x, offsets, counts, row_map=None, packed=False):
         """x rows grouped by expert (device-side `offsets`/`counts`, int64 [E], covering every
         row) -> FFN output rows, stored at `row_map[r]` instead of r when a map is given."""
-        return grouped_swiglu_ffn(x, self.w_gate_up, self.w_down, offsets, counts, row_map, covers_all_rows=True)
+        return grouped_swiglu_ffn(x, self.w_gate_up, self.w_down, offsets, counts, row_map, covers_all_rows=True,
+                                  packed=packed)  # fmt: skip
 
 
 class MoEFeedForward(nn.Module):
     grouped_gelu_min_experts = 16  # local GELU experts from which the FAST bf16 path runs them grouped
 
-    def __init__(self, dim, ff_dim, num_experts, top_k, implementation, group=None, expert_type="gelu"):
+    def __init__(self, dim, ff_dim, num_experts, top_k, implementation, group=None, expert_type="gelu",
+                 pack_activations=False):  # fmt: skip
         super().__init__()
+        if pack_activations and implementation != consts.MoEImplementation.FAST:
+            raise ValueError("pack_activations needs the FAST implementation (the grouped experts)")
+        self.pack_activations = pack_activations
         self.dim, self.num_experts, self.top_k = dim, num_experts, top_k
         self.implementation, self.group = implementation, group
         if dist.is_initialized():
@@ -243,7 +320,7 @@ class MoEFeedForward(nn.Module):
         offsets = torch.cumsum(counts, 0) - counts
         row_map = getattr(tokens_per_expert, "to_expert_major", None) if arrival_order_out else None
         if self.expert_type == "swiglu":
-            return self.experts(recv_data, offsets, counts, row_map)
+            return self.experts(recv_data, offsets, counts, row_map, self.pack_activations)
         # the reference's experts (nn.ModuleList of Linear-GELU-Linear, tiny_model.py:68-77): their
         # weights are stacked into the [E, N, K] layout the grouped GEMM reads; gradients flow
         # back to the individual modules through the stack
@@ -251,7 +328,8 @@ class MoEFeedForward(nn.Module):
         w2 = torch.stack([expert[2].weight for expert in self.experts])
         if w1.dtype != torch.bfloat16:  # bf16 autocast over fp32 modules: cast as autocast's linear would
             recv_data, w1, w2 = recv_data.bfloat16(), w1.bfloat16(), w2.bfloat16()
-        return grouped_gelu_ffn(recv_data, w1, w2, offsets, counts, row_map, covers_all_rows=True)
+        return grouped_gelu_ffn(recv_data, w1, w2, offsets, counts, row_map, covers_all_rows=True,
+                                packed=self.pack_activations)  # fmt: skip
 
     @staticmethod
     def _autocast_bf16():
@@ -269,7 +347,8 @@ class MoEFeedForward(nn.Module):
         # as per-expert library products and need no stacked copy of the weights (measured 259 ms
         # per step in the loop against 282 ms grouped), so everything else keeps the modules,
         # exactly as the reference runs them
-        if len(self.experts) < self.grouped_gelu_min_experts:
+        # (unless their activations are to be packed, which only the grouped experts do)
+        if len(self.experts) < self.grouped_gelu_min_experts and not self.pack_activations:
             return False
         fc1 = self.experts[0][0].weight
         in_bf16 = fc1.dtype == torch.bfloat16 and recv_data.dtype == torch.bfloat16
@@ -351,6 +430,10 @@ class MoEFeedForward(nn.Module):
         (again on every rank)."""
         from ..ep_fused import FusedExpertParallel
 
+        if self.pack_activations:
+            raise ValueError("the fused exchange keeps its activations in its own buffers: pack_activations is not served")
+        if self.is_int8:
+            raise ValueError("the fused exchange moves bf16 rows: it does not serve a layer in int8")
         self._fused_exchange = FusedExpertParallel(self, max_tokens, capacity_factor, self.group, expert_groups)
         return self
 
@@ -358,7 +441,55 @@ class MoEFeedForward(nn.Module):
         self._fused_exchange = None
         return self
 
-    def forward(self, x):
+    @property
+    def is_int8(self):
+        return getattr(self, "w1_q", None) is not None
+
+    def quantize_int8(self):
+        """From now on `forward` runs the experts in 8-bit integers (kernels/int8.py), for inference: the
+        weights are quantised here, once, with a scale per output channel. The router stays as it is.
+        The floating-point weights are kept; `dequantize()` returns to them. Single rank only."""
+        if self.world_size > 1 or getattr(self, "_fused_exchange", None) is not None:
+            raise ValueError("experts in int8 run on a single rank: rows do not travel in 8 bits")
+        if self.expert_type == "swiglu":
+            w1, w2 = int8.quantize_weight(self.experts.w_gate_up), int8.quantize_weight(self.experts.w_down)
+        else:
+            w1 = int8.quantize_weight(torch.stack([expert[0].weight.detach() for expert in self.experts]))
+            w2 = int8.quantize_weight(torch.stack([expert[2].weight.detach() for expert in self.experts]))
+        for name, w in (("w1", w1), ("w2", w2)):
+            self.register_buffer(f"{name}_q", w.q, persistent=False)
+            self.register_buffer(f"{name}_scale", w.scale, persistent=False)
+        return self
+
+    def dequantize(self):
+        for name in ("w1_q", "w1_scale", "w2_q", "w2_scale"):
+            if name in self._buffers:
+                del self._buffers[name]
+        return self
+
+    def _forward_int8(self, x, rows):
+        """The layer with its experts in 8 bits: every token's row is quantised once (or arrives
+        quantised, `rows`), and its int8 bytes and scale are what the dispatch copies top_k times."""
+        if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
+            raise ValueError("experts in int8 have no gradient: run them under torch.no_grad(), or dequantize() the layer")
+        B, T, D = x.shape
+        x_flat = x.reshape(-1, D)
+        topk_w, topk_idx = routing.route_topk(self.router(x_flat), self.top_k, w_dtype=x.dtype)
+        ix = routing.build_index(topk_idx, topk_w, self.num_experts)
+        if rows is None:
+            rows = int8.quantize_rows(x_flat)
+        rows = routing.permute_int8_rows(rows, ix, self.top_k)
+        ffn = int8.grouped_swiglu_ffn_int8 if self.expert_type == "swiglu" else int8.grouped_gelu_ffn_int8
+        w1, w2 = int8.Int8Weight(self.w1_q, self.w1_scale), int8.Int8Weight(self.w2_q, self.w2_scale)
+        out = ffn(rows, w1, w2, ix.offsets, ix.counts, covers_all_rows=True, out_dtype=x.dtype)
+        return self.unpermute(out, ix.reverse_map, ix.sorted_w, RoutedShape((B, T), ix.slot_of))
+
+    def forward(self, x, rows=None):
+        """`rows`: x in 8 bits, where a norm has produced it, for a layer in int8."""
+        if self.is_int8:
+            return self._forward_int8(x, rows)
+        if rows is not None:
+            raise ValueError("8-bit rows are for a layer in int8 (quantize_int8)")
         fused = getattr(self, "_fused_exchange", None)
         if fused is not None:
             needs_grad = torch.is_grad_enabled() and (
@@ -385,38 +516,75 @@ class FeedForward(nn.Module):
         self.fc1 = nn.Linear(dim, ff_dim, bias=False)
         self.fc2 = nn.Linear(ff_dim, dim, bias=False)
 
-    def forward(self, x):
-        return self.fc2(F.gelu(self.fc1(x)))
+    @property
+    def is_int8(self):
+        return isinstance(self.fc1, Int8Linear)
+
+    def quantize_int8(self):
+        """Both products in 8 bits, for inference."""
+        if not self.is_int8:
+            self.fc1, self.fc2 = Int8Linear(self.fc1), Int8Linear(self.fc2)
+        return self
+
+    def forward(self, x, rows=None):
+        return self.fc2(F.gelu(self.fc1(x) if rows is None else self.fc1(x, rows)))
+
+
+def _attend_and_norm(block, x, ff):
+    """The first half of a pre-norm block: (second norm's rows, their 8-bit form for a feed-forward `ff`
+    in int8 or None, stream = x + attention). With RMS norms the residual sum, the norm and the
+    quantisation are one pass over the rows."""
+    if not isinstance(block.norm1, RMSNorm):
+        x = x + block.attn(block.norm1(x))
+        return block.norm2(x), None, x
+    a = block.attn(x, block.norm1.int8(x).rows) if block.attn.is_int8 else block.attn(block.norm1(x))
+    if ff.is_int8:
+        n = block.norm2.int8(a, residual=x, with_y=True)
+        return n.y, n.rows, n.stream
+    y, x = block.norm2(a, x)
+    return y, None, x
+
+
+def _feed_forward(ff, y, rows):
+    return ff(y) if rows is None else ff(y, rows)
 
 
 class _ResidualBlock(nn.Module):
     """Pre-norm attention and feed-forward with residual connections; `self.ff` is set by the subclass."""
 
-    def __init__(self, dim, n_heads):
+    def __init__(self, dim, n_heads, norm="layer"):
         super().__init__()
-        self.norm1 = nn.LayerNorm(dim)
+        self.norm1 = _make_norm(norm, dim)
         self.attn = MultiheadSelfAttention(dim, n_heads)
-        self.norm2 = nn.LayerNorm(dim)
+        self.norm2 = _make_norm(norm, dim)
+
+    def quantize_int8(self):
+        """Attention projections and feed-forward in 8 bits, for inference."""
+        self.ff.quantize_int8()  # first: it is the one that may refuse
+        self.attn.quantize_int8()
+        return self
 
     def forward(self, x):
-        x = x + self.attn(self.norm1(x))
-        return x + self.ff(self.norm2(x))
+        y, rows, x = _attend_and_norm(self, x, self.ff)
+        return x + _feed_forward(self.ff, y, rows)
 
 
 class Block(_ResidualBlock):
     """Dense transformer block (tiny_model.py:424-435)."""
 
-    def __init__(self, dim, n_heads, ff_dim):
-        super().__init__(dim, n_heads)
+    def __init__(self, dim, n_heads, ff_dim, norm="layer"):
+        super().__init__(dim, n_heads, norm)
         self.ff = FeedForward(dim, ff_dim)
 
 
 class MoEBlock(_ResidualBlock):
     """Transformer block whose feed-forward is a `MoEFeedForward` (tiny_model.py:438-463)."""
 
-    def __init__(self, dim, n_heads, ff_dim, num_experts, top_k, implementation, expert_type="gelu"):
-        super().__init__(dim, n_heads)
-        self.ff = MoEFeedForward(dim, ff_dim, num_experts, top_k, implementation, expert_type=expert_type)
+    def __init__(self, dim, n_heads, ff_dim, num_experts, top_k, implementation, expert_type="gelu", norm="layer",
+                 pack_activations=False):  # fmt: skip
+        super().__init__(dim, n_heads, norm)
+        self.ff = MoEFeedForward(dim, ff_dim, num_experts, top_k, implementation, expert_type=expert_type,
+                                 pack_activations=pack_activations)  # fmt: skip
 
 
 class PipelinedMoEBlock(nn.Module):
@@ -429,13 +597,14 @@ class PipelinedMoEBlock(nn.Module):
     overlap, and splitting the batch only doubles the per-expert launches."""
 
     def __init__(self, dim, n_heads, ff_dim, num_experts, top_k, stream0, stream1,
-                 comm_balance_factor=1, num_micro_batches=None, expert_type="gelu"):  # fmt: skip
+                 comm_balance_factor=1, num_micro_batches=None, expert_type="gelu", norm="layer",
+                 pack_activations=False):  # fmt: skip
         super().__init__()
-        self.norm1 = nn.LayerNorm(dim)
+        self.norm1 = _make_norm(norm, dim)
         self.attn = MultiheadSelfAttention(dim, n_heads)
-        self.norm2 = nn.LayerNorm(dim)
+        self.norm2 = _make_norm(norm, dim)
         self.moe = MoEFeedForward(dim, ff_dim, num_experts, top_k, consts.MoEImplementation.FAST,
-                                  expert_type=expert_type)  # fmt: skip
+                                  expert_type=expert_type, pack_activations=pack_activations)  # fmt: skip
         self.stream0, self.stream1 = stream0, stream1
         self.comm_balance_factor = comm_balance_factor  # kept for signature parity; padding is never sent
         self.num_micro_batches = num_micro_batches
@@ -451,15 +620,22 @@ class PipelinedMoEBlock(nn.Module):
             self._extra_streams.append(torch.cuda.Stream())
         return (streams + self._extra_streams)[:n]
 
+    def quantize_int8(self):
+        """Attention projections and experts in 8 bits, for inference (single rank)."""
+        self.moe.quantize_int8()  # first: it is the one that may refuse
+        self.attn.quantize_int8()
+        return self
+
     def forward(self, x):
         n_mb = self.num_micro_batches
         if n_mb is None:
             n_mb = 2 if self.moe.world_size > 1 else 1
-        if n_mb == 1 or getattr(self.moe, "_fused_exchange", None) is not None:
-            # nothing to overlap here: one micro-batch, or the fused exchange, which overlaps the
-            # dispatch of one expert group with the GEMMs of the previous one inside the layer
-            x = x + self.attn(self.norm1(x))
-            return x + self.moe(self.norm2(x))
+        if n_mb == 1 or getattr(self.moe, "_fused_exchange", None) is not None or self.moe.is_int8:
+            # nothing to overlap here: one micro-batch, a single rank's int8 layer, or the fused
+            # exchange, which overlaps the dispatch of one expert group with the GEMMs of the
+            # previous one inside the layer
+            y, rows, x = _attend_and_norm(self, x, self.moe)
+            return x + _feed_forward(self.moe, y, rows)
         chunks = x.chunk(n_mb, dim=0)
         streams = self._streams(len(chunks))
         main = torch.cuda.current_stream()
@@ -472,9 +648,9 @@ class PipelinedMoEBlock(nn.Module):
                 if prev_attn_done is not None:
                     s.wait_event(prev_attn_done)
                 with record_function(f"S{i}: Attn {i}"):
-                    r = mb + self.attn(self.norm1(mb))
+                    y, _, r = _attend_and_norm(self, mb, self.moe)
                     resid.append(r)
-                    moe_in.append(self.norm2(r))
+                    moe_in.append(y)
                 prev_attn_done = torch.cuda.Event()
                 prev_attn_done.record()
         moe_out = pipelined_moe_forward(self.moe, moe_in, streams)
@@ -547,7 +723,8 @@ class TinyModel(nn.Module):
 
     def __init__(self, in_dim, dim, n_heads, ff_dim, n_layers, num_experts=None, top_k=None,
                  implementation=None, stream0=None, stream1=None, comm_balance_factor=1, *,
-                 use_moe, expert_type="gelu", num_micro_batches=None):  # fmt: skip
+                 use_moe, expert_type="gelu", num_micro_batches=None, norm="layer",
+                 pack_activations=False):  # fmt: skip
         super().__init__()
         self.inp = nn.Linear(in_dim, dim, bias=False)
         if use_moe:
@@ -555,18 +732,29 @@ class TinyModel(nn.Module):
                 raise ValueError("use_moe=True needs num_experts")
             top_k = 2 if top_k is None else top_k
         if not use_moe:
-            blocks = [Block(dim, n_heads, ff_dim) for _ in range(n_layers)]
+            if pack_activations:
+                raise ValueError("pack_activations is for experts: it needs use_moe=True")
+            blocks = [Block(dim, n_heads, ff_dim, norm) for _ in range(n_layers)]
         elif implementation == consts.MoEImplementation.STANDARD:
-            blocks = [MoEBlock(dim, n_heads, ff_dim, num_experts, top_k, implementation, expert_type)
+            blocks = [MoEBlock(dim, n_heads, ff_dim, num_experts, top_k, implementation, expert_type, norm,
+                               pack_activations)
                       for _ in range(n_layers)]  # fmt: skip
         elif implementation == consts.MoEImplementation.FAST:
             blocks = [PipelinedMoEBlock(dim, n_heads, ff_dim, num_experts, top_k, stream0, stream1,
-                                        comm_balance_factor, num_micro_batches, expert_type)
+                                        comm_balance_factor, num_micro_batches, expert_type, norm, pack_activations)
                       for _ in range(n_layers)]  # fmt: skip
         else:
             raise NotImplementedError(f"implementation {implementation!r}")
         self.blocks = nn.ModuleList(blocks)
         self.out = nn.Linear(dim, in_dim, bias=False)
+
+    def quantize_int8(self):
+        """Every block's products in 8-bit integers, for inference (single rank); the input and output
+        projections stay as they are. To be called on the model where and as it will run: a later
+        cast of the module's floating-point buffers would also cast the scales, which a product refuses."""
+        for block in self.blocks:
+            block.quantize_int8()
+        return self
 
     def forward(self, x):
         x = self.inp(x)
