@@ -18,6 +18,44 @@ constexpr uint32_t kInfBits = 0x7f800000u;
 // magnitudes, with infinity and NaN above every finite value, so a maximum never loses a NaN.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+// Adding this to |t| < 2^22 rounds t to a whole number (nearest, ties to even) and leaves that number's
+// two's complement in the low bits of the sum. Conversion instructions run at an eighth of the rate of
+// an addition, too few for the values that HBM delivers.
+constexpr float kRounder = 12582912.f;  // 1.5 * 2^23
+constexpr float kNear = 0.5f - 3e-5f;
+
+// Two fp32 operations in one instruction (sm_100's packed fp32 forms; the rounding is that of each).
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+      "fma.rn.f32x2 rd, ra, rb, rc;\n\t"
+      "mov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rd, ra, rb;\n\t"
+      "mov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mul.rn.f32x2 rd, ra, rb;\n\t"
+      "mov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 struct Quantiser {
   float top;    // a
   float inv;    // 127 / a
@@ -29,24 +67,81 @@ struct Quantiser {
     inv = __fdiv_rn(127.f, top);
     scale = fine ? __fdiv_rn(top, 127.f) : __uint_as_float(0x7fc00000u);
   }
-  // v * (127 / a) in fp32 is off by at most 127 * 2 * 2^-24 = 1.6e-5: only a quotient that close
-  // to the border between two whole numbers is taken again in 64 bits (6 in 100000 values).
-  __device__ __forceinline__ int operator()(float v) const {
-    const float t = v * inv;
-    float r = rintf(t);
-    if (fabsf(t - r) > 0.5f - 3e-5f) r = static_cast<float>(rint(static_cast<double>(v) * 127.0 / static_cast<double>(top)));
-    return fine ? static_cast<int>(r) : 0;
+  // N values: words[i] holds q of v[4 i .. 4 i + 3] (N = 1: of v[0], in the low byte). The budget is
+  // tight: three bytes of DRAM traffic per 16-bit value leave eight instructions for it, so the
+  // arithmetic goes in pairs.
+  template <int N>
+  __device__ __forceinline__ void operator()(const float* v, uint32_t* words) const {
+    float s[N];
+    float off = 0.f;  // largest distance between a quotient and the whole number it went to
+    if constexpr (N == 1) {
+      s[0] = fmaf(v[0], inv, kRounder);
+      off = fabsf(fmaf(v[0], inv, -(s[0] - kRounder)));
+    } else {
+      const float2 inv2 = make_float2(inv, inv), up = make_float2(kRounder, kRounder);
+      const float2 down = make_float2(-kRounder, -kRounder), minus = make_float2(-1.f, -1.f);
+#pragma unroll
+      for (int j = 0; j < N; j += 2) {
+        const float2 x = make_float2(v[j], v[j + 1]);
+        const float2 t = fma2(x, inv2, up);
+        const float2 d = fma2(x, inv2, mul2(add2(t, down), minus));
+        s[j] = t.x;
+        s[j + 1] = t.y;
+        off = fmaxf(off, fmaxf(fabsf(d.x), fabsf(d.y)));
+      }
+    }
+    // v * (127 / a) is off by at most 127 * 2 * 2^-24 = 1.6e-5. A quotient that lies that close to the
+    // border between two whole numbers is compared with the border exactly. (One in 16000 of
+    // arbitrary values does; among 16-bit values one that is exactly a / 2, at 63.5, is common.)
+    if (off > kNear) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float r = s[j] - kRounder, d = fmaf(v[j], inv, -r);
+        if (fabsf(d) > kNear) {
+          // The border next to r on d's side is m / 2 with m = 2 r +- 1; the side of v is the sign of
+          // 254 v - m a, both taken times 2^-8 against overflow. m a = h + low exactly; 254 v - h and
+          // the difference that is left have 18 bits or fewer in units of v's last one: exact too.
+          const float sign = copysignf(1.f, d);
+          const float m = fmaf(2.f, r, sign) * 0x1p-8f;
+          const float h = m * top, low = fmaf(m, top, -h);
+          const float side = (fmaf(v[j], 254.f / 256.f, -h) - low) * sign;
+          if (side > 0.f || (side == 0.f && (__float_as_uint(s[j]) & 1u))) s[j] += sign;
+        }
+      }
+    }
+    if constexpr (N == 1) {
+      words[0] = fine ? __float_as_uint(s[0]) & 255u : 0u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; j += 4) {
+        const uint32_t lo = __byte_perm(__float_as_uint(s[j]), __float_as_uint(s[j + 1]), 0x0040);
+        const uint32_t hi = __byte_perm(__float_as_uint(s[j + 2]), __float_as_uint(s[j + 3]), 0x0040);
+        words[j / 4] = fine ? __byte_perm(lo, hi, 0x5410) : 0u;
+      }
+    }
   }
 };
 
-__device__ __forceinline__ uint32_t pack_int8(int a, int b, int c, int d) {
-  return (a & 255) | ((b & 255) << 8) | ((c & 255) << 16) | (static_cast<uint32_t>(d) << 24);
+// Bits of the largest |v| of a 16-byte vector of DT (see abs_bits), NaN if one is NaN.
+template <int DT>
+__device__ __forceinline__ uint32_t vec_top(const uint4& v, uint32_t top) {
+  if constexpr (DT == FMOE_F32) {
+    return max(max(top, max(v.x & 0x7fffffffu, v.y & 0x7fffffffu)), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+  } else {  // two 16-bit magnitudes to a word: unsigned order again, in each half
+    const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+    const uint16_t b = static_cast<uint16_t>(max(m & 0xffffu, m >> 16));
+    float f;
+    if constexpr (DT == FMOE_BF16) f = __uint_as_float(static_cast<uint32_t>(b) << 16);
+    else f = __half2float(__ushort_as_half(b));
+    return max(top, abs_bits(f));
+  }
 }
 
-// Four int8 in a word as floats.
+// Four int8 in a word as floats: v + 128 goes into the last bits of 2^23, no conversion either.
 __device__ __forceinline__ void unpack_int8(uint32_t w, float* f) {
+  w ^= 0x80808080u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
+  for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 + i)) - 8388736.f;
 }
 
 #endif  // __CUDACC__

@@ -6,7 +6,7 @@
 //   SwiGLU   from h~ = [gate | up] and grad: d_gate, d_up, and hidden = silu(gate) * up again,
 //            which the down projection's weight gradient needs and the forward need not keep
 //   GELU     the same for hidden = gelu(h~)
-// All are single streaming passes bound by HBM: 16 lanes share a group, eight columns each.
+// All are single streaming passes bound by HBM.
 #include "int8.cuh"
 #include "tcgen05.cuh"
 
@@ -50,34 +50,51 @@ __device__ __forceinline__ void load8_packed(const int8_t* row, int64_t c, float
   for (int j = 0; j < 8; ++j) f[j] *= s;
 }
 
+// Eight lanes share a group, sixteen columns each.
 template <int DT>
 __global__ void __launch_bounds__(256) pack_kernel(const void* x, int64_t x_stride, int8_t* q, int64_t q_stride,
                                                    float* scale, int64_t T, int64_t D, int groups, int vec) {
   using E = typename Elem<DT>::type;
+  constexpr int VE = Elem<DT>::kVec;
   const int64_t total = T * groups;
-  const int sub = threadIdx.x & 15;
-  // both halves of a warp stay in the loop together: the shuffles below need all 32 lanes
-  for (int64_t g0 = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 5) * 2; g0 < total;
-       g0 += static_cast<int64_t>(gridDim.x) * 16) {
-    const int64_t g = g0 + ((threadIdx.x >> 4) & 1);
+  const int sub = threadIdx.x & 7;
+  // the four groups of a warp stay in the loop together: the shuffles below need all 32 lanes
+  for (int64_t g0 = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x >> 5) * 4; g0 < total;
+       g0 += static_cast<int64_t>(gridDim.x) * 32) {
+    const int64_t g = g0 + ((threadIdx.x >> 3) & 3);
     const bool live = g < total;
     const int64_t row = live ? g / groups : 0;
     const int k = static_cast<int>(g - row * groups);
-    const int64_t c = static_cast<int64_t>(k) * kGroup + sub * 8;
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (live && c < D) load8<DT>(static_cast<const E*>(x) + row * x_stride, c, D, vec, f);
+    const int64_t c = static_cast<int64_t>(k) * kGroup + sub * 16;
+    const E* p = static_cast<const E*>(x) + row * x_stride + c;
+    uint4 v[16 / VE];
     uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, abs_bits(f[j]));
+    for (int i = 0; i < 16 / VE; ++i) {
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (live && c + i * VE < D) {
+        if (vec) {
+          v[i] = ld_stream16(reinterpret_cast<const uint4*>(p + i * VE));
+        } else {
+          float f[VE];
 #pragma unroll
-    for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+          for (int j = 0; j < VE; ++j) f[j] = c + i * VE + j < D ? to_float<DT>(p[i * VE + j]) : 0.f;
+          v[i] = pack16<DT>(f);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16 / VE; ++i) top = vec_top<DT>(v[i], top);
+#pragma unroll
+    for (int d = 4; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
     const Quantiser quant(top);
     if (live && c < q_stride) {  // past D: zeros up to the 16-byte step
-      int r[8];
+      float f[16];
+      uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = quant(f[j]);
-      *reinterpret_cast<uint2*>(q + row * q_stride + c) =
-          make_uint2(pack_int8(r[0], r[1], r[2], r[3]), pack_int8(r[4], r[5], r[6], r[7]));
+      for (int i = 0; i < 16 / VE; ++i) unpack16<DT>(v[i], f + i * VE);
+      quant.operator()<16>(f, w);
+      st_stream16(reinterpret_cast<uint4*>(q + row * q_stride + c), make_uint4(w[0], w[1], w[2], w[3]));
     }
     if (live && sub == 0) scale[row * groups + k] = quant.scale;
   }
@@ -97,7 +114,9 @@ __global__ void __launch_bounds__(256) unpack_kernel(const int8_t* q, int64_t q_
   }
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
+// The fast exponential and quotient are off by (2 + |x|) and 2 steps of 2^-23: the result goes into
+// products that are rounded to 16 bits, or held to a 32-bit bound that counts them.
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
 // One thread: eight columns of the gate half and the same columns of the up half. A width that is
 // not a multiple of eight leaves the up half's bytes off the 8-byte grid: they are read one by one.
@@ -185,7 +204,7 @@ extern "C" int fmoe_pack_activation(const void* x, int64_t x_stride, int8_t* q, 
   FMOE_REQUIRE(T == 1 || x_stride >= D, FMOE_ERR_ARG, "fmoe_pack_activation: the row stride must be at least D");
   const int groups = packed_groups(D);
   const int vec = D % 8 == 0 && aligned_to(x, 16) && x_stride * dtype_size(dtype) % 16 == 0;
-  FMOE_DISPATCH_DTYPE(dtype, DT, pack_kernel<DT><<<stream_grid((T * groups + 15) / 16), 256, 0,
+  FMOE_DISPATCH_DTYPE(dtype, DT, pack_kernel<DT><<<stream_grid((T * groups + 31) / 32), 256, 0,
                                                    static_cast<cudaStream_t>(stream)>>>(x, x_stride, q, q_stride, scale, T,
                                                                                         D, groups, vec));
   return check_launch("pack_kernel");

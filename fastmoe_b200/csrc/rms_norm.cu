@@ -28,52 +28,118 @@ struct RowArgs {
   int64_t x_stride, r_stride, q_stride;
   double eps;
   int w_f32;
+  int shift0, shift_step;  // see row_shift
 };
 
-// ---- loads and stores of VE elements -----------------------------------------------------------
-template <int DT, int VE>
-struct Vec {  // VE elements of 16 bytes in all
+// ---- a row as 16-byte vectors, wherever it starts ------------------------------------------------
+// A row of odd width starts anywhere on the 2- or 4-byte grid. What matters for wide accesses is that
+// all tensors of a call are off the 16-byte grid by the same number of elements in a given row,
+// which contiguous tensors of one shape are: the row is then cut at the grid, vector c holds the
+// elements c * VE - shift + (0 .. VE - 1), and only the first and the last one may be partial.
+__device__ __forceinline__ int row_shift(int shift0, int shift_step, int64_t row, int VE) {
+  return (shift0 + static_cast<int>(row & (VE - 1)) * shift_step) & (VE - 1);
+}
+
+// The partial vectors, one at each end of a shifted row. Out of line: inlined into the unrolled loops
+// they cost 100 registers a thread that every other vector pays for.
+template <int DT>
+__device__ __noinline__ uint4 load_partial(const typename Elem<DT>::type* row, int e, int D) {
+  float f[Elem<DT>::kVec];
+#pragma unroll
+  for (int j = 0; j < Elem<DT>::kVec; ++j) f[j] = e + j >= 0 && e + j < D ? to_float<DT>(row[e + j]) : 0.f;
+  return pack16<DT>(f);
+}
+template <int DT>
+__device__ __noinline__ void store_partial(typename Elem<DT>::type* row, int e, int D, uint4 v) {
+  float f[Elem<DT>::kVec];
+  unpack16<DT>(v, f);
+#pragma unroll
+  for (int j = 0; j < Elem<DT>::kVec; ++j)
+    if (e + j >= 0 && e + j < D) row[e + j] = from_float<DT>(f[j]);
+}
+
+// How the kernels cut rows: rows that start on the grid and end on it, shifted rows, or (tensors that
+// are off the grid by different amounts) one element at a time.
+enum Cut { kAligned, kShifted, kSingle };
+
+// Elements e .. e + kElems - 1 of a row of D, in registers as they lie in memory; those outside the row are zeros.
+template <int DT, int CUT>
+struct Vec {
+  using E = typename Elem<DT>::type;
+  static constexpr int kElems = Elem<DT>::kVec;
   uint4 v;
-  __device__ __forceinline__ void load(const void* p, int64_t i) {
-    v = ld_stream16(reinterpret_cast<const uint4*>(static_cast<const typename Elem<DT>::type*>(p) + i));
+  __device__ __forceinline__ static bool whole(int e, int D) { return CUT == kAligned || (e >= 0 && e + kElems <= D); }
+  __device__ __forceinline__ void load(const E* row, int e, int D) {
+    if (whole(e, D)) v = ld_stream16(reinterpret_cast<const uint4*>(row + e));
+    else v = load_partial<DT>(row, e, D);
   }
+  __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void get(float* f) const { unpack16<DT>(v, f); }
   __device__ __forceinline__ void set(const float* f) { v = pack16<DT>(f); }
-  __device__ __forceinline__ void store(void* p, int64_t i) const {
-    *reinterpret_cast<uint4*>(static_cast<typename Elem<DT>::type*>(p) + i) = v;
+  __device__ __forceinline__ void store(E* row, int e, int D) const {
+    if (whole(e, D)) *reinterpret_cast<uint4*>(row + e) = v;
+    else store_partial<DT>(row, e, D, v);
   }
+  __device__ __forceinline__ uint32_t top(uint32_t t) const { return vec_top<DT>(v, t); }
 };
 template <int DT>
-struct Vec<DT, 1> {  // one element
-  typename Elem<DT>::type v;
-  __device__ __forceinline__ void load(const void* p, int64_t i) { v = static_cast<const typename Elem<DT>::type*>(p)[i]; }
+struct Vec<DT, kSingle> {
+  using E = typename Elem<DT>::type;
+  static constexpr int kElems = 1;
+  E v;
+  __device__ __forceinline__ void load(const E* row, int e, int) { v = row[e]; }
+  __device__ __forceinline__ void zero() { v = from_float<DT>(0.f); }
   __device__ __forceinline__ void get(float* f) const { f[0] = to_float<DT>(v); }
   __device__ __forceinline__ void set(const float* f) { v = from_float<DT>(f[0]); }
-  __device__ __forceinline__ void store(void* p, int64_t i) const { static_cast<typename Elem<DT>::type*>(p)[i] = v; }
+  __device__ __forceinline__ void store(E* row, int e, int) const { row[e] = v; }
+  __device__ __forceinline__ uint32_t top(uint32_t t) const { return max(t, abs_bits(to_float<DT>(v))); }
 };
 
-// VE weights, fp32 or of the rows' type, as floats.
-template <int DT, int VE>
-__device__ __forceinline__ void load_weight(const void* w, int w_f32, int64_t i, float* f) {
-  if constexpr (VE == 1) {
-    f[0] = w_f32 ? static_cast<const float*>(w)[i] : to_float<DT>(static_cast<const typename Elem<DT>::type*>(w)[i]);
-  } else if (w_f32) {
+// Weights e .. e + VE - 1, fp32 or of the rows' type, as floats; zeros outside the row. The weight
+// starts on the grid (w_vec) whatever the row does, so in a shifted row its elements are read one by one,
+// out of L1.
+template <int DT, int CUT>
+__device__ __forceinline__ void load_weight(const void* w, int w_f32, int e, int D, float* f) {
+  using E = typename Elem<DT>::type;
+  constexpr int VE = Vec<DT, CUT>::kElems;
+  if (CUT == kAligned || (CUT == kShifted && (e & (VE - 1)) == 0 && e + VE <= D)) {
+    if constexpr (CUT != kSingle) {
+      if (w_f32) {
 #pragma unroll
-    for (int j = 0; j < VE; j += 4)
-      unpack16<FMOE_F32>(ld_cached16(reinterpret_cast<const uint4*>(static_cast<const float*>(w) + i + j)), f + j);
+        for (int j = 0; j < VE; j += 4)
+          unpack16<FMOE_F32>(ld_cached16(reinterpret_cast<const uint4*>(static_cast<const float*>(w) + e + j)), f + j);
+      } else {
+        unpack16<DT>(ld_cached16(reinterpret_cast<const uint4*>(static_cast<const E*>(w) + e)), f);
+      }
+    }
   } else {
-    unpack16<DT>(ld_cached16(reinterpret_cast<const uint4*>(static_cast<const typename Elem<DT>::type*>(w) + i)), f);
+#pragma unroll
+    for (int j = 0; j < VE; ++j) {
+      f[j] = 0.f;
+      if (e + j >= 0 && e + j < D)
+        f[j] = w_f32 ? static_cast<const float*>(w)[e + j] : to_float<DT>(static_cast<const E*>(w)[e + j]);
+    }
   }
 }
 
-template <int VE>
-__device__ __forceinline__ void store_int8(int8_t* p, const int* r) {
-  if constexpr (VE == 8)
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_int8(r[0], r[1], r[2], r[3]), pack_int8(r[4], r[5], r[6], r[7]));
-  else if constexpr (VE == 4)
-    *reinterpret_cast<uint32_t*>(p) = pack_int8(r[0], r[1], r[2], r[3]);
-  else
-    *p = static_cast<int8_t>(r[0]);
+// q of elements e .. to a row of 8-bit values, which starts on the grid: in the widest pieces that the
+// shift leaves aligned.
+template <int VE, int CUT>
+__device__ __forceinline__ void store_int8(int8_t* row, int e, int D, const uint32_t* words) {
+  if constexpr (VE == 1) {
+    row[e] = static_cast<int8_t>(words[0]);
+  } else if (CUT == kAligned || (e >= 0 && e + VE <= D && (e & (VE - 1)) == 0)) {
+    if constexpr (VE == 8) *reinterpret_cast<uint2*>(row + e) = make_uint2(words[0], words[1]);
+    else *reinterpret_cast<uint32_t*>(row + e) = words[0];
+  } else if (e >= 0 && e + VE <= D && (e & 1) == 0) {
+#pragma unroll
+    for (int j = 0; j < VE / 2; ++j)
+      *reinterpret_cast<uint16_t*>(row + e + 2 * j) = static_cast<uint16_t>(words[j / 2] >> (16 * (j & 1)));
+  } else {
+#pragma unroll
+    for (int j = 0; j < VE; ++j)
+      if (e + j >= 0 && e + j < D) row[e + j] = static_cast<int8_t>(words[j / 4] >> (8 * (j & 3)));
+  }
 }
 
 // ---- reductions over the threads of a row: a warp, or the whole CTA ----------------------------
@@ -114,90 +180,107 @@ __device__ __forceinline__ float inv_rms(double sum_sq, int64_t D, double eps) {
 constexpr int row_threads(int elements) { return elements > 8 ? 512 : 1024; }
 
 // One row per CTA, or per warp (WARP: narrow rows, threadIdx.y picks the row), each thread holding
-// VPT vectors of VE elements of it in registers.
-template <int DT, int VE, int VPT, bool WARP, bool NORM>
-__global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * VE)) row_kernel(const RowArgs a) {
+// VPT vectors of it in registers, as they lie in memory: what is unpacked twice costs fewer cycles
+// than the CTAs that 32 fp32 registers a thread would keep off the SM.
+template <int DT, int CUT, int VPT, bool WARP, bool NORM>
+__global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::kElems)) row_kernel(const RowArgs a) {
   __shared__ double part_sum[32];
   __shared__ uint32_t part_max[32];
+  constexpr int VE = Vec<DT, CUT>::kElems;
   const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y : blockIdx.x;
   if (row >= a.T) return;  // WARP only: no barrier follows
   const int tid = threadIdx.x, nthr = WARP ? 32 : blockDim.x;
-  const int nvec = static_cast<int>(a.D / VE);
+  const int D = static_cast<int>(a.D);
   using E = typename Elem<DT>::type;
-  const E* x = static_cast<const E*>(a.x) + row * a.x_stride;
+  const int first = tid * VE - (CUT == kShifted ? row_shift(a.shift0, a.shift_step, row, VE) : 0);  // this thread's first element
+  const int step = nthr * VE;
 
-  float v[VPT][VE];
+  Vec<DT, CUT> sv[VPT];
   {
-    Vec<DT, VE> xv[VPT], rv[VPT];
+    const E* x = static_cast<const E*>(a.x) + row * a.x_stride;
     const E* r = static_cast<const E*>(a.residual) + row * a.r_stride;
+    Vec<DT, CUT> rv[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = i * nthr + tid;
-      if (c < nvec) {
-        xv[i].load(x, static_cast<int64_t>(c) * VE);
-        if (a.residual != nullptr) rv[i].load(r, static_cast<int64_t>(c) * VE);
+      const int e = first + i * step;
+      if (e < D) {
+        sv[i].load(x, e, D);
+        if (NORM && a.residual != nullptr) rv[i].load(r, e, D);
+      } else {
+        sv[i].zero();
       }
     }
+    if (NORM && a.residual != nullptr) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = i * nthr + tid;
-      if (c < nvec) {
-        xv[i].get(v[i]);
-        if (a.residual != nullptr) {
-          float f[VE];
-          rv[i].get(f);
+      for (int i = 0; i < VPT; ++i) {
+        const int e = first + i * step;
+        if (e < D) {
+          float f[VE], g[VE];
+          sv[i].get(f);
+          rv[i].get(g);
 #pragma unroll
-          for (int j = 0; j < VE; ++j) f[j] += v[i][j];
-          rv[i].set(f);  // the one rounding of the sum
-          rv[i].store(static_cast<E*>(a.sum) + row * a.D, static_cast<int64_t>(c) * VE);
-          rv[i].get(v[i]);
+          for (int j = 0; j < VE; ++j) f[j] += g[j];
+          sv[i].set(f);  // the one rounding of the sum
+          sv[i].store(static_cast<E*>(a.sum) + row * a.D, e, D);
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < VE; ++j) v[i][j] = 0.f;
       }
     }
   }
+  uint32_t top = 0;
+  float rstd = 1.f;
   if constexpr (NORM) {
     double sq = 0.0;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int j = 0; j < VE; ++j) sq = fma(static_cast<double>(v[i][j]), static_cast<double>(v[i][j]), sq);
-    const float rstd = inv_rms(row_sum<WARP>(sq, part_sum), a.D, a.eps);
-    if (a.rstd != nullptr && tid == 0) a.rstd[row] = rstd;
-#pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = i * nthr + tid;
-      if (c < nvec) {
-        float w[VE];
-        load_weight<DT, VE>(a.w, a.w_f32, static_cast<int64_t>(c) * VE, w);
+      float f[VE];
+      sv[i].get(f);
 #pragma unroll
-        for (int j = 0; j < VE; ++j) v[i][j] = v[i][j] * rstd * w[j];
+      for (int j = 0; j < VE; ++j) sq = fma(static_cast<double>(f[j]), static_cast<double>(f[j]), sq);
+    }
+    rstd = inv_rms(row_sum<WARP>(sq, part_sum), a.D, a.eps);
+    if (a.rstd != nullptr && tid == 0) a.rstd[row] = rstd;
+  }
+  auto value = [&](int i, float* f) {
+    sv[i].get(f);
+    if constexpr (NORM) {
+      float w[VE];
+      load_weight<DT, CUT>(a.w, a.w_f32, first + i * step, D, w);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) f[j] = f[j] * rstd * w[j];
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int e = first + i * step;
+    if (e < D) {
+      if constexpr (NORM) {
+        float f[VE];
+        value(i, f);
         if (a.y != nullptr) {
-          Vec<DT, VE> out;
-          out.set(v[i]);
-          out.store(static_cast<E*>(a.y) + row * a.D, static_cast<int64_t>(c) * VE);
+          Vec<DT, CUT> out;
+          out.set(f);
+          out.store(static_cast<E*>(a.y) + row * a.D, e, D);
         }
+        // elements outside the row are zeros, or NaN where the row is not finite
+#pragma unroll
+        for (int j = 0; j < VE; ++j) top = max(top, abs_bits(f[j]));
+      } else {
+        top = sv[i].top(top);
       }
     }
   }
   if (a.q == nullptr) return;
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i)
-#pragma unroll
-    for (int j = 0; j < VE; ++j) top = max(top, i * nthr + tid < nvec ? abs_bits(v[i][j]) : 0u);
   const Quantiser quant(row_max<WARP>(top, part_max));
   int8_t* q = a.q + row * a.q_stride;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int c = i * nthr + tid;
-    if (c < nvec) {
-      int r[VE];
-#pragma unroll
-      for (int j = 0; j < VE; ++j) r[j] = quant(v[i][j]);
-      store_int8<VE>(q + static_cast<int64_t>(c) * VE, r);
+    const int e = first + i * step;
+    if (e < D) {
+      float f[VE];
+      uint32_t words[(VE + 3) / 4];
+      value(i, f);
+      quant.template operator()<VE>(f, words);
+      store_int8<VE, CUT>(q, e, D, words);
     }
   }
   const int pad = static_cast<int>((16 - (a.D & 15)) & 15);  // up to the next 16 bytes: zeros
@@ -212,10 +295,11 @@ __global__ void __launch_bounds__(1024) row_loop_kernel(const RowArgs a) {
   __shared__ uint32_t part_max[32];
   using E = typename Elem<DT>::type;
   const int64_t row = blockIdx.x;
+  const int D = static_cast<int>(a.D);
   const E* x = static_cast<const E*>(a.x) + row * a.x_stride;
   E* sum = static_cast<E*>(a.sum) + row * a.D;
   double sq = 0.0;
-  for (int64_t c = threadIdx.x; c < a.D; c += blockDim.x) {
+  for (int c = threadIdx.x; c < D; c += blockDim.x) {
     float f = to_float<DT>(x[c]);
     if (a.residual != nullptr) {
       const E s = from_float<DT>(f + to_float<DT>(static_cast<const E*>(a.residual)[row * a.r_stride + c]));
@@ -229,17 +313,17 @@ __global__ void __launch_bounds__(1024) row_loop_kernel(const RowArgs a) {
     rstd = inv_rms(row_sum<false>(sq, part_sum), a.D, a.eps);
     if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = rstd;
   }
-  auto value = [&](int64_t c) {
+  auto value = [&](int c) {
     float f = to_float<DT>(a.residual != nullptr ? sum[c] : x[c]);
     if constexpr (NORM) {
       float w;
-      load_weight<DT, 1>(a.w, a.w_f32, c, &w);
+      load_weight<DT, kSingle>(a.w, a.w_f32, c, D, &w);
       f = f * rstd * w;
     }
     return f;
   };
   uint32_t top = 0;
-  for (int64_t c = threadIdx.x; c < a.D; c += blockDim.x) {
+  for (int c = threadIdx.x; c < D; c += blockDim.x) {
     const float f = value(c);
     if (a.y != nullptr) static_cast<E*>(a.y)[row * a.D + c] = from_float<DT>(f);
     top = max(top, abs_bits(f));
@@ -247,7 +331,12 @@ __global__ void __launch_bounds__(1024) row_loop_kernel(const RowArgs a) {
   if (a.q == nullptr) return;
   const Quantiser quant(row_max<false>(top, part_max));
   int8_t* q = a.q + row * a.q_stride;
-  for (int64_t c = threadIdx.x; c < a.D; c += blockDim.x) q[c] = static_cast<int8_t>(quant(value(c)));
+  for (int c = threadIdx.x; c < D; c += blockDim.x) {
+    const float f = value(c);
+    uint32_t word;
+    quant.operator()<1>(&f, &word);
+    q[c] = static_cast<int8_t>(word);
+  }
   const int pad = static_cast<int>((16 - (a.D & 15)) & 15);
   if (threadIdx.x < pad) q[a.D + threadIdx.x] = 0;
   if (threadIdx.x == 0) a.q_scale[row] = quant.scale;
@@ -265,49 +354,83 @@ struct RowBwdArgs {
   int64_t T, D;
   int64_t dy_stride, ds_stride, s_stride;
   int w_f32;
+  int shift0, shift_step;
 };
 
 // A CTA (or each of its warps) walks rows t, t + grid, ... and keeps its columns' share of dw in
 // registers; the shares are added by rms_dw_kernel in a fixed order, so dw has the same bits from
-// run to run.
-template <int DT, int VE, int VPT, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * VE)) rms_bwd_kernel(const RowBwdArgs a) {
+// run to run. Rows of one thread are a multiple of VE apart, so that their shift is the same and a
+// thread's columns stay its own. The weight lies in shared memory as fp32, in the CTA's shifted
+// order and in planes of four columns (16-byte reads without bank conflicts).
+template <int DT, int CUT, int VPT, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::kElems)) rms_bwd_kernel(const RowBwdArgs a) {
   __shared__ float part_sum[2][32];
+  extern __shared__ __align__(16) float w_smem[];
+  constexpr int VE = Vec<DT, CUT>::kElems;
   using E = typename Elem<DT>::type;
   const int tid = threadIdx.x, nthr = WARP ? 32 : blockDim.x;
-  const int nvec = static_cast<int>(a.D / VE);
+  const int D = static_cast<int>(a.D);
   const int rows_per_cta = WARP ? blockDim.y : 1;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_per_cta + (WARP ? threadIdx.y : 0);
+  const int first = tid * VE - (CUT == kShifted ? row_shift(a.shift0, a.shift_step, row0, VE) : 0);
+  const int step = nthr * VE;
+  constexpr int kPlanes = VE >= 4 ? VE / 4 : 1, kWide = VE >= 4 ? 4 : 1;
+  const int plane = nthr * VPT * kWide;  // floats per plane
+  if constexpr (!WARP) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float w[VE];
+#pragma unroll
+      for (int j = 0; j < VE; ++j) w[j] = 0.f;
+      if (first + i * step < D) load_weight<DT, CUT>(a.w, a.w_f32, first + i * step, D, w);
+#pragma unroll
+      for (int p = 0; p < kPlanes; ++p)
+#pragma unroll
+        for (int j = 0; j < kWide; ++j) w_smem[p * plane + (i * nthr + tid) * kWide + j] = w[p * kWide + j];
+    }
+  }  // each thread reads back what it wrote itself: no barrier
+  auto weight = [&](int i, float* w) {
+    if constexpr (WARP) {
+      load_weight<DT, CUT>(a.w, a.w_f32, first + i * step, D, w);
+    } else if constexpr (VE >= 4) {
+#pragma unroll
+      for (int p = 0; p < kPlanes; ++p) {
+        const float4 q = *reinterpret_cast<const float4*>(w_smem + p * plane + (i * nthr + tid) * 4);
+        w[4 * p] = q.x, w[4 * p + 1] = q.y, w[4 * p + 2] = q.z, w[4 * p + 3] = q.w;
+      }
+    } else {
+      w[0] = w_smem[i * nthr + tid];
+    }
+  };
   float dw[VPT][VE];
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
 #pragma unroll
     for (int j = 0; j < VE; ++j) dw[i][j] = 0.f;
   int flip = 0;  // two sets of partial sums: a row's first write never meets the last row's reads
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * rows_per_cta + (WARP ? threadIdx.y : 0); row < a.T;
-       row += static_cast<int64_t>(gridDim.x) * rows_per_cta, flip ^= 1) {
+  for (int64_t row = row0; row < a.T; row += static_cast<int64_t>(gridDim.x) * rows_per_cta, flip ^= 1) {
     const E* s = static_cast<const E*>(a.s) + row * a.s_stride;
     const E* dy = static_cast<const E*>(a.dy) + row * a.dy_stride;
     const E* ds = static_cast<const E*>(a.ds) + row * a.ds_stride;
-    Vec<DT, VE> sv[VPT], gv[VPT], dv[VPT];
+    Vec<DT, CUT> sv[VPT], gv[VPT], dv[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = i * nthr + tid;
-      if (c < nvec) {
-        sv[i].load(s, static_cast<int64_t>(c) * VE);
-        gv[i].load(dy, static_cast<int64_t>(c) * VE);
-        if (a.ds != nullptr) dv[i].load(ds, static_cast<int64_t>(c) * VE);
+      const int e = first + i * step;
+      if (e < D) {
+        sv[i].load(s, e, D);
+        gv[i].load(dy, e, D);
+        if (a.ds != nullptr) dv[i].load(ds, e, D);
       }
     }
     const float rstd = a.rstd[row];
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = i * nthr + tid;
-      if (c < nvec) {
+      if (first + i * step < D) {
         float xh[VE], g[VE], w[VE];
         sv[i].get(xh);
         gv[i].get(g);
-        load_weight<DT, VE>(a.w, a.w_f32, static_cast<int64_t>(c) * VE, w);
+        weight(i, w);
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
           const float t = g[j] * (xh[j] * rstd);
@@ -319,49 +442,47 @@ __global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * VE)) rms_bwd_ke
     const float mean = row_sum<WARP>(dot, part_sum[flip]) / static_cast<float>(a.D);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = i * nthr + tid;
-      if (c < nvec) {
+      const int e = first + i * step;
+      if (e < D) {
         float xh[VE], g[VE], w[VE], d[VE];
         sv[i].get(xh);
         gv[i].get(g);
-        load_weight<DT, VE>(a.w, a.w_f32, static_cast<int64_t>(c) * VE, w);
+        weight(i, w);
 #pragma unroll
         for (int j = 0; j < VE; ++j) d[j] = 0.f;
         if (a.ds != nullptr) dv[i].get(d);
 #pragma unroll
         for (int j = 0; j < VE; ++j) d[j] = fmaf(rstd, fmaf(-(xh[j] * rstd), mean, g[j] * w[j]), d[j]);
-        Vec<DT, VE> out;
+        Vec<DT, CUT> out;
         out.set(d);
-        out.store(static_cast<E*>(a.dx) + row * a.D, static_cast<int64_t>(c) * VE);
+        out.store(static_cast<E*>(a.dx) + row * a.D, e, D);
       }
     }
   }
   if (a.part == nullptr) return;
   float* part = a.part + static_cast<int64_t>(blockIdx.x) * a.D;
   if constexpr (WARP) {  // the CTA's warps, one after the other
-    __shared__ float acc[32 * VPT * VE];
     for (int y = 0; y < blockDim.y; ++y) {
       if (threadIdx.y == y) {
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
           for (int j = 0; j < VE; ++j) {
-            const int k = (i * 32 + tid) * VE + j;
-            acc[k] = y == 0 ? dw[i][j] : acc[k] + dw[i][j];
+            const int e = first + i * step + j;
+            if (e >= 0 && e < D) w_smem[e] = y == 0 ? dw[i][j] : w_smem[e] + dw[i][j];
           }
       }
       __syncthreads();
     }
-    for (int k = threadIdx.y * 32 + tid; k < a.D; k += blockDim.y * 32) part[k] = acc[k];
+    for (int e = threadIdx.y * 32 + tid; e < D; e += blockDim.y * 32) part[e] = w_smem[e];
   } else {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = i * nthr + tid;
-      if (c < nvec) {
+    for (int i = 0; i < VPT; ++i)
 #pragma unroll
-        for (int j = 0; j < VE; ++j) part[static_cast<int64_t>(c) * VE + j] = dw[i][j];
+      for (int j = 0; j < VE; ++j) {
+        const int e = first + i * step + j;
+        if (e >= 0 && e < D) part[e] = dw[i][j];
       }
-    }
   }
 }
 
@@ -370,6 +491,7 @@ template <int DT>
 __global__ void __launch_bounds__(1024) rms_bwd_loop_kernel(const RowBwdArgs a) {
   __shared__ float part_sum[2][32];
   using E = typename Elem<DT>::type;
+  const int D = static_cast<int>(a.D);
   float* part = a.part == nullptr ? nullptr : a.part + static_cast<int64_t>(blockIdx.x) * a.D;
   int flip = 0;
   bool first = true;
@@ -378,18 +500,18 @@ __global__ void __launch_bounds__(1024) rms_bwd_loop_kernel(const RowBwdArgs a) 
     const E* dy = static_cast<const E*>(a.dy) + row * a.dy_stride;
     const float rstd = a.rstd[row];
     float dot = 0.f;
-    for (int64_t c = threadIdx.x; c < a.D; c += blockDim.x) {
+    for (int c = threadIdx.x; c < D; c += blockDim.x) {
       float w;
-      load_weight<DT, 1>(a.w, a.w_f32, c, &w);
+      load_weight<DT, kSingle>(a.w, a.w_f32, c, D, &w);
       const float t = to_float<DT>(dy[c]) * (to_float<DT>(s[c]) * rstd);
       if (part != nullptr) part[c] = first ? t : part[c] + t;  // this thread alone has this column
       dot = fmaf(t, w, dot);
     }
     first = false;
     const float mean = row_sum<false>(dot, part_sum[flip]) / static_cast<float>(a.D);
-    for (int64_t c = threadIdx.x; c < a.D; c += blockDim.x) {
+    for (int c = threadIdx.x; c < D; c += blockDim.x) {
       float w;
-      load_weight<DT, 1>(a.w, a.w_f32, c, &w);
+      load_weight<DT, kSingle>(a.w, a.w_f32, c, D, &w);
       const float d = a.ds == nullptr ? 0.f : to_float<DT>(static_cast<const E*>(a.ds)[row * a.ds_stride + c]);
       const float v = fmaf(rstd, fmaf(-(to_float<DT>(s[c]) * rstd), mean, to_float<DT>(dy[c]) * w), d);
       static_cast<E*>(a.dx)[row * a.D + c] = from_float<DT>(v);
@@ -443,23 +565,45 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* q, int64_
 }
 
 // ---- host side ------------------------------------------------------------------------------
-// How a row is split: 16-byte vectors where widths, strides and addresses allow, else single
-// elements; a warp per row while a row fits 32 threads, else a CTA. A CTA takes four vectors a
+// The shift of row r is (shift0 + r * shift_step) mod VE (row_shift) if all tensors of the call agree on
+// it; `vec` says whether they do.
+struct RowGrid {
+  int ve, shift0 = -1, shift_step = 0;
+  bool vec = true;
+  RowGrid(int dtype) : ve(16 / dtype_size(dtype)), es(dtype_size(dtype)) {}
+  void add(const void* p, int64_t stride, int64_t T) {
+    if (p == nullptr) return;
+    const int s0 = static_cast<int>(reinterpret_cast<uintptr_t>(p) / es % ve);
+    const int st = T > 1 ? static_cast<int>(stride % ve) : 0;
+    if (reinterpret_cast<uintptr_t>(p) % es != 0 || (shift0 >= 0 && (s0 != shift0 || st != shift_step))) vec = false;
+    shift0 = s0;
+    shift_step = st;
+  }
+  void weight(const void* w) { vec = vec && aligned_to(w, 16); }
+  bool shifted() const { return vec && (shift0 != 0 || shift_step != 0); }
+
+ private:
+  int es;
+};
+
+// How a row is split: a warp per row while a row fits 32 threads, else a CTA. A CTA takes four vectors a
 // thread when there are rows enough to fill the GPU (more loads in flight per thread), one or two
 // when there are not (the latency of a single row falls with the vectors per thread).
 struct RowShape {
-  bool vec, warp, loop;
+  Cut cut;
+  bool warp, loop;
   int vpt, threads;
 };
-static RowShape row_shape(bool vec, int64_t D, int64_t T, int dtype) {
-  RowShape s{vec, false, false, 0, 0};
-  const int ve = vec ? 16 / dtype_size(dtype) : 1;
+static RowShape row_shape(const RowGrid& g, int64_t D, int64_t T, int dtype) {
+  const bool vec = g.vec;
+  RowShape s{!vec ? kSingle : g.shifted() || D % g.ve != 0 ? kShifted : kAligned, false, false, 0, 0};
+  const int ve = vec ? g.ve : 1;
   const int most = vec ? (dtype == FMOE_F32 ? 8 : 4) : 16;  // vectors a thread can hold: 32 elements, or 16 single ones
-  const int64_t nvec = D / ve;
-  if (nvec <= 32 * (vec ? 4 : 16)) {
+  const int64_t nvec = (D + (g.shifted() ? ve - 1 : 0) + ve - 1) / ve;  // of the row with the largest shift
+  if (nvec <= 32 * (vec ? 2 : 16)) {
     s.warp = true;
     s.threads = 32;
-    s.vpt = vec ? (nvec <= 32 ? 1 : nvec <= 64 ? 2 : 4) : 16;
+    s.vpt = vec ? (nvec <= 32 ? 1 : 2) : 16;
     return s;
   }
   s.vpt = T <= 2 * kNumSMs ? (vec ? 1 : 4) : (vec ? 4 : 16);
@@ -469,58 +613,70 @@ static RowShape row_shape(bool vec, int64_t D, int64_t T, int dtype) {
   return s;
 }
 
+// The instantiation for RowShape s, through FMOE_ROWS(CUT, VPT, WARP).
+#define FMOE_PICK_ROWS                                                   \
+  do {                                                                   \
+    if (s.cut == kSingle) {                                              \
+      if (s.warp) FMOE_ROWS(kSingle, 16, true);                          \
+      else if (s.vpt == 4) FMOE_ROWS(kSingle, 4, false);                 \
+      else FMOE_ROWS(kSingle, 16, false);                                \
+    } else if (s.cut == kAligned) {                                      \
+      FMOE_PICK_VPT(kAligned);                                           \
+    } else {                                                             \
+      FMOE_PICK_VPT(kShifted);                                           \
+    }                                                                    \
+  } while (0)
+#define FMOE_PICK_VPT(CUT)                                               \
+  do {                                                                   \
+    if (s.warp && s.vpt == 1) FMOE_ROWS(CUT, 1, true);                   \
+    else if (s.warp) FMOE_ROWS(CUT, 2, true);                            \
+    else if (s.vpt == 1) FMOE_ROWS(CUT, 1, false);                       \
+    else if (s.vpt == 2) FMOE_ROWS(CUT, 2, false);                       \
+    else if (s.vpt == 4) FMOE_ROWS(CUT, 4, false);                       \
+    else if constexpr (Elem<DT>::kVec == 4) FMOE_ROWS(CUT, 8, false);    \
+  } while (0)
+
 template <int DT, bool NORM>
 static int launch_rows(const RowArgs& a, const RowShape& s, cudaStream_t st) {
-  constexpr int V = Elem<DT>::kVec;
   const dim3 block = s.warp ? dim3(32, a.T >= 8 * kNumSMs ? 8 : 1) : dim3(s.threads);
   const unsigned grid = static_cast<unsigned>(s.warp ? (a.T + block.y - 1) / block.y : a.T);
-#define FMOE_ROWS(VE, VPT, WARP) row_kernel<DT, VE, VPT, WARP, NORM><<<grid, block, 0, st>>>(a)
+#define FMOE_ROWS(CUT, VPT, WARP) row_kernel<DT, CUT, VPT, WARP, NORM><<<grid, block, 0, st>>>(a)
   if (s.loop) row_loop_kernel<DT, NORM><<<grid, 1024, 0, st>>>(a);
-  else if (!s.vec && s.warp) FMOE_ROWS(1, 16, true);
-  else if (!s.vec && s.vpt == 4) FMOE_ROWS(1, 4, false);
-  else if (!s.vec) FMOE_ROWS(1, 16, false);
-  else if (s.warp && s.vpt == 1) FMOE_ROWS(V, 1, true);
-  else if (s.warp && s.vpt == 2) FMOE_ROWS(V, 2, true);
-  else if (s.warp) FMOE_ROWS(V, 4, true);
-  else if (s.vpt == 1) FMOE_ROWS(V, 1, false);
-  else if (s.vpt == 2) FMOE_ROWS(V, 2, false);
-  else if (s.vpt == 4) FMOE_ROWS(V, 4, false);
-  else if constexpr (V == 4) FMOE_ROWS(V, 8, false);
+  else FMOE_PICK_ROWS;
 #undef FMOE_ROWS
   return check_launch(NORM ? "row_kernel (norm)" : "row_kernel (quantize)");
 }
 
+constexpr int kBwdWarps = 8;  // rows per CTA where a warp takes a row
+
 template <int DT>
 static int launch_bwd(const RowBwdArgs& a, const RowShape& s, int grid, cudaStream_t st) {
   constexpr int V = Elem<DT>::kVec;
-  const dim3 block = s.warp ? dim3(32, 8) : dim3(s.threads);
-#define FMOE_ROWS(VE, VPT, WARP) rms_bwd_kernel<DT, VE, VPT, WARP><<<grid, block, 0, st>>>(a)
+  const dim3 block = s.warp ? dim3(32, kBwdWarps) : dim3(s.threads);
+  const int smem = static_cast<int>(sizeof(float)) * (s.warp ? static_cast<int>(a.D) : s.threads * s.vpt * (s.cut == kSingle ? 1 : V));
+  cudaError_t err = cudaSuccess;
+#define FMOE_ROWS(CUT, VPT, WARP)                                                                                \
+  do {                                                                                                           \
+    if (smem > 48 * 1024)                                                                                        \
+      err = cudaFuncSetAttribute(rms_bwd_kernel<DT, CUT, VPT, WARP>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
+                                 smem);                                                                          \
+    if (err == cudaSuccess) rms_bwd_kernel<DT, CUT, VPT, WARP><<<grid, block, smem, st>>>(a);                     \
+  } while (0)
   if (s.loop) rms_bwd_loop_kernel<DT><<<grid, 1024, 0, st>>>(a);
-  else if (!s.vec && s.warp) FMOE_ROWS(1, 16, true);
-  else if (!s.vec && s.vpt == 4) FMOE_ROWS(1, 4, false);
-  else if (!s.vec) FMOE_ROWS(1, 16, false);
-  else if (s.warp && s.vpt == 1) FMOE_ROWS(V, 1, true);
-  else if (s.warp && s.vpt == 2) FMOE_ROWS(V, 2, true);
-  else if (s.warp) FMOE_ROWS(V, 4, true);
-  else if (s.vpt == 1) FMOE_ROWS(V, 1, false);
-  else if (s.vpt == 2) FMOE_ROWS(V, 2, false);
-  else if (s.vpt == 4) FMOE_ROWS(V, 4, false);
-  else if constexpr (V == 4) FMOE_ROWS(V, 8, false);
+  else FMOE_PICK_ROWS;
 #undef FMOE_ROWS
+  FMOE_CUDA(err);
   return check_launch("rms_bwd_kernel");
 }
 
-// CTAs of the backward pass, and so shares of dw: enough to fill the GPU, each with a few rows.
-static int bwd_grid(int64_t T, int64_t D) {
-  const int64_t per_sm = D <= 1024 ? 4 : D <= 2048 ? 8 : D <= 4096 ? 4 : 2;
-  const int64_t rows = D <= 1024 ? (T + 7) / 8 : T;  // the narrowest rows run eight to a CTA
-  const int64_t most = per_sm * kNumSMs;
-  return static_cast<int>(rows < most ? (rows > 0 ? rows : 1) : most);
+// CTAs of the backward pass, and so shares of dw: as many as the SMs hold at a time, a multiple of eight
+// (see rms_bwd_kernel). The size query does not know the shape that runs: it answers for the most.
+static int bwd_grid(int64_t T, int64_t D, bool warp) {
+  const int64_t per_sm = warp ? 4 : D <= 2048 ? 8 : D <= 4096 ? 4 : 2;
+  const int64_t rows = warp ? (T + kBwdWarps - 1) / kBwdWarps : T, most = per_sm * kNumSMs;
+  return static_cast<int>(rows < most ? rows : most);
 }
-
-static bool rows16(const void* p, int64_t stride, int dtype) {
-  return aligned_to(p, 16) && stride * dtype_size(dtype) % 16 == 0;
-}
+static_assert(kNumSMs * 2 % 8 == 0, "rows of one CTA must be a multiple of 8 apart");
 
 }  // namespace fmoe
 
@@ -543,10 +699,15 @@ extern "C" int fmoe_rms_norm(const void* x, int64_t x_stride, const void* residu
   FMOE_REQUIRE((q == nullptr) == (q_scale == nullptr), FMOE_ERR_ARG, "fmoe_rms_norm: q and q_scale come together");
   FMOE_REQUIRE(!q || (q_stride % 16 == 0 && q_stride >= D && aligned_to(q, 16)), FMOE_ERR_ARG,
                "fmoe_rms_norm: 8-bit rows must lie at 16-byte steps");
-  const bool vec = D % (16 / dtype_size(dtype)) == 0 && rows16(x, x_stride, dtype) && aligned_to(w, 16) &&
-                   (!residual || (rows16(residual, r_stride, dtype) && aligned_to(sum, 16))) && (!y || aligned_to(y, 16));
-  const RowArgs a{x, residual, w, y, sum, rstd, q, q_scale, T, D, x_stride, r_stride, q_stride, eps, w_dtype == FMOE_F32};
-  const RowShape s = row_shape(vec, D, T, dtype);
+  RowGrid g(dtype);
+  g.add(x, x_stride, T);
+  g.add(residual, r_stride, T);
+  g.add(sum, D, T);
+  g.add(y, D, T);
+  g.weight(w);
+  const RowArgs a{x, residual, w, y, sum, rstd, q, q_scale, T, D, x_stride, r_stride, q_stride, eps, w_dtype == FMOE_F32,
+                  g.shift0, g.shift_step};
+  const RowShape s = row_shape(g, D, T, dtype);
   int rc = FMOE_OK;
   FMOE_DISPATCH_DTYPE(dtype, DT, rc = (launch_rows<DT, true>(a, s, static_cast<cudaStream_t>(stream))));
   return rc;
@@ -562,9 +723,11 @@ extern "C" int fmoe_quantize_rows(const void* x, int64_t x_stride, int8_t* q, in
   FMOE_REQUIRE(T == 1 || x_stride >= D, FMOE_ERR_ARG, "fmoe_quantize_rows: the row stride must be at least D");
   FMOE_REQUIRE(q_stride % 16 == 0 && q_stride >= D && aligned_to(q, 16), FMOE_ERR_ARG,
                "fmoe_quantize_rows: 8-bit rows must lie at 16-byte steps");
-  const bool vec = D % (16 / dtype_size(dtype)) == 0 && rows16(x, x_stride, dtype);
-  const RowArgs a{x, nullptr, nullptr, nullptr, nullptr, nullptr, q, q_scale, T, D, x_stride, 0, q_stride, 0.0, 0};
-  const RowShape s = row_shape(vec, D, T, dtype);
+  RowGrid g(dtype);
+  g.add(x, x_stride, T);
+  const RowArgs a{x, nullptr, nullptr, nullptr, nullptr, nullptr, q, q_scale, T, D, x_stride, 0, q_stride, 0.0, 0,
+                  g.shift0, g.shift_step};
+  const RowShape s = row_shape(g, D, T, dtype);
   int rc = FMOE_OK;
   FMOE_DISPATCH_DTYPE(dtype, DT, rc = (launch_rows<DT, false>(a, s, static_cast<cudaStream_t>(stream))));
   return rc;
@@ -590,7 +753,7 @@ extern "C" int fmoe_dequantize_rows(const int8_t* q, int64_t q_stride, const flo
 
 extern "C" size_t fmoe_rms_norm_bwd_bytes(int64_t T, int64_t D) {
   if (T <= 0 || D <= 0) return 0;
-  return static_cast<size_t>(bwd_grid(T, D)) * static_cast<size_t>(D) * sizeof(float);
+  return static_cast<size_t>(bwd_grid(T, D, false)) * static_cast<size_t>(D) * sizeof(float);
 }
 
 extern "C" int fmoe_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dsum, int64_t ds_stride, const void* sum,
@@ -610,12 +773,16 @@ extern "C" int fmoe_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* 
                "fmoe_rms_norm_bwd: row strides must be at least D");
   FMOE_REQUIRE(!dw || (scratch && aligned_to(scratch, 4) && scratch_bytes >= fmoe_rms_norm_bwd_bytes(T, D)),
                FMOE_ERR_WORKSPACE, "fmoe_rms_norm_bwd: scratch of %zu bytes needed", fmoe_rms_norm_bwd_bytes(T, D));
-  const bool vec = D % (16 / dtype_size(dtype)) == 0 && rows16(dy, dy_stride, dtype) && rows16(sum, s_stride, dtype) &&
-                   (!dsum || rows16(dsum, ds_stride, dtype)) && aligned_to(w, 16) && aligned_to(dx, 16);
-  const RowShape s = row_shape(vec, D, T, dtype);
-  const int grid = bwd_grid(T, D);
+  RowGrid g(dtype);
+  g.add(dy, dy_stride, T);
+  g.add(sum, s_stride, T);
+  g.add(dsum, ds_stride, T);
+  g.add(dx, D, T);
+  g.weight(w);
+  const RowShape s = row_shape(g, D, T, dtype);
+  const int grid = bwd_grid(T, D, s.warp);
   const RowBwdArgs a{dy, dsum, sum, rstd, w, dx, dw ? static_cast<float*>(scratch) : nullptr, T, D,
-                     dy_stride, ds_stride, s_stride, w_dtype == FMOE_F32};
+                     dy_stride, ds_stride, s_stride, w_dtype == FMOE_F32, g.shift0, g.shift_step};
   int rc = FMOE_OK;
   FMOE_DISPATCH_DTYPE(dtype, DT, rc = (launch_bwd<DT>(a, s, grid, st)));
   if (rc != 0 || dw == nullptr) return rc;
