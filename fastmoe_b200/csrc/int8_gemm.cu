@@ -6,13 +6,13 @@
 // result does not depend on how K is split or in which order parts arrive; the two scales are
 // applied in fp32 and the result is rounded once.
 //
-// int8_gemm_kernel, per CTA (192 threads, one CTA per SM):
+// int8_gemm_kernel, per CTA (320 threads, one CTA per SM):
 //   warp 0      TMA producer: A tile 128 x 128 bytes and W tile 256 x 128 bytes per stage, 128-byte
 //               swizzle, 4 stages, mbarrier full/empty pairs; rows and columns past the ends of
 //               the tensors read as zeros, so R, N and K need not be multiples of the tile
 //   warp 1      MMA issuer: one thread issues tcgen05.mma (M=128, N=256, K=32, s8 x s8 -> s32) into
 //               one of two 256-column TMEM accumulators
-//   warps 2-5   epilogue: tcgen05.ld, integer -> float, scales, activation, stores of the valid
+//   warps 2-9   epilogue: tcgen05.ld, integer -> float, scales, activation, stores of the valid
 //               rows and columns while the next tile's MMAs fill the other accumulator
 // Every mbarrier wait is bounded, as in grouped_gemm.cu.
 #include "int8.cuh"
@@ -28,8 +28,10 @@ constexpr int kBM = 128, kBN = 256, kBK = 128, kStages = 4, kUmmaK = 32;
 constexpr int kABytes = kBM * kBK;  // 16 KB
 constexpr int kBBytes = kBN * kBK;  // 32 KB
 constexpr int kStageBytes = kABytes + kBBytes;
-constexpr int kThreads = 192;
-constexpr int kEpiStageBytes = 4 * 32 * 128;  // one 32-row x 128-byte block per epilogue warp
+constexpr int kThreads = 192;      // int8_tn_kernel
+constexpr int kEpiWarps = 8;       // of int8_gemm_kernel: two per quarter of tensor memory, half of the columns each
+constexpr int kTileThreads = 64 + 32 * kEpiWarps;
+constexpr int kEpiStageBytes = kEpiWarps * 32 * 64;  // one 32-row x 64-byte block per epilogue warp
 constexpr int kMaxExperts = 1024;
 constexpr int kRowGroup = 16;  // row blocks that share their column blocks' weight tiles, see locate()
 
@@ -106,7 +108,7 @@ __device__ __forceinline__ Tile locate(int tile, const int* mb_prefix, const Arg
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kTileThreads, 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                      const Args a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -129,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool mma_issued = false;
 
   // ---- set-up: tile table, barriers, TMEM ----------------------------------------------
-  for (int e = threadIdx.x; e < a.E; e += kThreads) {
+  for (int e = threadIdx.x; e < a.E; e += kTileThreads) {
     const int64_t n = rows_of(a, e);
     if (a.counts != nullptr && n != a.counts[e] && a.counts[e] > 0 && a.status != nullptr && blockIdx.x == 0)
       atomicOr(a.status, FMOE_STATUS_BAD_EXPERT);  // rows past the end of A were cut off
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tmem_full[i], 1);
-      mbar_init(&tmem_empty[i], 4);
+      mbar_init(&tmem_empty[i], kEpiWarps);
     }
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -224,9 +226,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- epilogue -------------------------------------------------------------------
     using E = typename Elem<DT>::type;
     constexpr int kPiece = Elem<DT>::kVec;  // columns per 16 bytes of C
-    constexpr int kChunk = 8 * kPiece;      // columns per 128-byte segment of a row of C: 64, or 32 in fp32
-    const int quarter = warp & 3;
-    uint4* stage_w = stage_buf + (warp - 2) * (32 * 8);
+    constexpr int kPart = 4 * kPiece;       // columns per 64-byte segment of a row of C: 32, or 16 in fp32
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    uint4* stage_w = stage_buf + (warp - 2) * (32 * 4);
     const int out_cols = swiglu ? 128 : kBN;
     int it = 0;
     for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++it) {
@@ -239,65 +241,66 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!mbar_wait(&tmem_full[acc], (it >> 1) & 1, abort_flag, a.spin_limit)) goto timed_out;
       tcgen05_fence_after();
       const uint32_t taddr = tmem_base + acc * kBN + (static_cast<uint32_t>(quarter * 32) << 16);
+      const int c_end = (half + 1) * (out_cols / 2);
 #pragma unroll 1
-      for (int c0 = 0; c0 < out_cols && warp_rows > 0; c0 += kChunk) {
+      for (int c0 = half * (out_cols / 2); c0 < c_end && warp_rows > 0; c0 += 32) {
         const int64_t col0 = static_cast<int64_t>(t.nb) * out_cols + c0;
-        const int cols = static_cast<int>(a.cols - col0 < kChunk ? a.cols - col0 : kChunk);
+        const int cols = static_cast<int>(a.cols - col0 < 32 ? a.cols - col0 : 32);
         if (cols <= 0) break;
+        float f[32];
+        // lane j holds the channel scale of column j and hands it round
+        const float s0 = lane < cols ? sw[col0 + lane] : 0.f;
+        if (swiglu) {
+          const float s1 = lane < cols ? sw[a.cols + col0 + lane] : 0.f;
+          uint32_t g[32], u[32];
+          tmem_ld32(taddr + c0, g);
+          tmem_ld32(taddr + 128 + c0, u);
+          tmem_ld_wait();
 #pragma unroll
-        for (int h = 0; h < kChunk / 32; ++h) {
-          float f[32];
-          // lane j holds the channel scale of column 32 h + j and hands it round
-          const int64_t mine = col0 + 32 * h + lane;
-          const float s0 = mine < a.cols ? sw[mine] : 0.f;
-          if (swiglu) {
-            const float s1 = mine < a.cols ? sw[a.cols + mine] : 0.f;
-            uint32_t g[32], u[32];
-            tmem_ld32(taddr + c0 + 32 * h, g);
-            tmem_ld32(taddr + 128 + c0 + 32 * h, u);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float gate = static_cast<float>(static_cast<int>(g[i])) * sa * __shfl_sync(0xffffffffu, s0, i);
-              const float up = static_cast<float>(static_cast<int>(u[i])) * sa * __shfl_sync(0xffffffffu, s1, i);
-              f[i] = silu(gate) * up;
-            }
-          } else {
-            uint32_t r[32];
-            tmem_ld32(taddr + c0 + 32 * h, r);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              f[i] = static_cast<float>(static_cast<int>(r[i])) * sa * __shfl_sync(0xffffffffu, s0, i);
-            if (a.act == FMOE_ACT_GELU) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) f[i] = gelu_erf(f[i]);
-            }
+          for (int i = 0; i < 32; ++i) {
+            const float gate = static_cast<float>(static_cast<int>(g[i])) * sa * __shfl_sync(0xffffffffu, s0, i);
+            const float up = static_cast<float>(static_cast<int>(u[i])) * sa * __shfl_sync(0xffffffffu, s1, i);
+            f[i] = gate * sigmoid(gate) * up;
           }
+        } else {
+          uint32_t r[32];
+          tmem_ld32(taddr + c0, r);
+          tmem_ld_wait();
 #pragma unroll
-          for (int v = 0; v < 32 / kPiece; ++v)
-            stage_w[lane * 8 + (((32 / kPiece) * h + v) ^ (lane & 7))] = pack16<DT>(f + kPiece * v);
-        }
-        __syncwarp();
-        // rows are regrouped through the swizzled staging block: four whole 128-byte segments a store
-        const int q = lane & 7, left = cols - q * kPiece;
+          for (int i = 0; i < 32; ++i)
+            f[i] = static_cast<float>(static_cast<int>(r[i])) * sa * __shfl_sync(0xffffffffu, s0, i);
+          if (a.act == FMOE_ACT_GELU) {
 #pragma unroll
-        for (int step = 0; step < 8; ++step) {
-          const int r = step * 4 + (lane >> 3);
-          if (r < warp_rows && left > 0) {
-            const uint4 val = stage_w[r * 8 + (q ^ (r & 7))];
-            E* p = static_cast<E*>(a.C) + (t.row0 + quarter * 32 + r) * a.cols + col0 + q * kPiece;
-            if (a.vec_ok && left >= kPiece) {
-              *reinterpret_cast<uint4*>(p) = val;
-            } else {
-              const E* from = reinterpret_cast<const E*>(&val);
-#pragma unroll
-              for (int j = 0; j < kPiece; ++j)
-                if (j < left) p[j] = from[j];
-            }
+            for (int i = 0; i < 32; ++i) f[i] = gelu(f[i]);
           }
         }
-        __syncwarp();
+        // rows are regrouped through a swizzled staging block: whole 64-byte segments a store
+#pragma unroll
+        for (int h = 0; h < 32 / kPart; ++h) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            stage_w[lane * 4 + (v ^ ((lane >> 1) & 3))] = pack16<DT>(f + h * kPart + kPiece * v);
+          __syncwarp();
+          E* out = static_cast<E*>(a.C) + (t.row0 + quarter * 32) * a.cols + col0 + h * kPart;
+          const int n = cols - h * kPart;
+          if (a.vec_ok && n >= kPart) {
+#pragma unroll
+            for (int step = 0; step < 4; ++step) {
+              const int r = step * 8 + (lane >> 2), q = lane & 3;
+              if (r < warp_rows)
+                *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r) * a.cols + q * kPiece) = stage_w[r * 4 + (q ^ ((r >> 1) & 3))];
+            }
+          } else {  // rows off the 16-byte grid, or the last columns: an element a lane
+            constexpr int kRows = 32 / kPart;  // rows a store covers: 1, or 2 in fp32
+            const int j = lane & (kPart - 1);
+#pragma unroll 4
+            for (int r = lane / kPart; r < warp_rows && r < 32; r += kRows) {
+              const E* from = reinterpret_cast<const E*>(&stage_w[r * 4 + ((j / kPiece) ^ ((r >> 1) & 3))]);
+              if (j < n) out[static_cast<int64_t>(r) * a.cols + j] = from[j & (kPiece - 1)];
+            }
+          }
+          __syncwarp();
+        }
       }
       tcgen05_fence_before();
       __syncwarp();
@@ -321,6 +324,532 @@ done:
   }
 }
 
+// ---- few rows per expert: weights streamed past a handful of tokens ------------------------------
+// With a few rows the product is bound by reading the weights once, and a 128 x 256 tile per CTA leaves
+// most SMs without one (21504 x 7168 weights are 84 tiles; 7168 x 7168 are 28). Here a CTA takes 32
+// weight rows and all of up to 8 * NT tokens, its eight warps each every eighth 128-byte piece of K:
+// weights are the 16-row operand of mma.sync m16n8k32 and go from global memory straight into its
+// fragments, tokens are the 8-column operand. A product's K order is free as long as both operands
+// agree, so a thread's fragment words are the 16 consecutive bytes that one load brings:
+// lane (g, t) takes bytes 16 t .. 16 t + 15 of a 64-byte step of rows g and g + 8, word 0 and 1 as
+// the first MMA's two k halves, word 2 and 3 as the second's. The warps' integer sums meet in shared
+// memory: exact, so the split changes nothing. The legacy MMA's rate does not matter here: it is the
+// tile shape that counts.
+constexpr int kFewThreads = 256, kFewWarps = 8, kFewRows = 32;  // weight rows per CTA
+constexpr int kFewStep = 128;                                  // bytes of K per warp and step
+constexpr int64_t kFewBytes = 16 << 20, kFewTokens = 256;  // weight bytes times passes, see fmoe_int8_gemm
+constexpr int kFewPad = 4;  // columns of padding in the reduction buffer: fragment stores without bank conflicts
+
+struct FewArgs {
+  const int8_t* A;
+  const int8_t* W;
+  int64_t a_stride, w_stride, w_expert_stride;
+  int64_t K;
+  int n_blocks;  // groups of 32 weight rows (16 gate + 16 up rows for SwiGLU) per expert
+  Args g;
+};
+
+__device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 bytes of a token from byte k on, with zeros from K on: what lies behind a row does not count.
+__device__ __forceinline__ uint4 load_token(const int8_t* row, int k, int K) {
+  if (row == nullptr || k >= K) return make_uint4(0, 0, 0, 0);
+  uint4 v = __ldg(reinterpret_cast<const uint4*>(row + k));
+  if (k + 16 > K) {
+    auto keep = [&](int i) { return K - k >= 4 * i + 4 ? ~0u : K - k <= 4 * i ? 0u : ~0u >> (32 - 8 * (K - k - 4 * i)); };
+    v.x &= keep(0), v.y &= keep(1), v.z &= keep(2), v.w &= keep(3);
+  }
+  return v;
+}
+
+template <int DT, int NT>
+__global__ void __launch_bounds__(kFewThreads) int8_few_rows_kernel(const FewArgs f) {
+  using E = typename Elem<DT>::type;
+  constexpr int kTokens = 8 * NT, kLine = kFewRows + kFewPad;
+  __shared__ int red[kFewWarps][kTokens][kLine];
+  extern __shared__ int chunk_prefix[];  // [E + 1] chunks of kTokens rows before each expert
+  const Args& a = f.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int K = static_cast<int>(f.K);
+  const bool swiglu = a.act == FMOE_ACT_SWIGLU;
+
+  for (int e = threadIdx.x; e < a.E; e += kFewThreads) {
+    const int64_t n = rows_of(a, e);
+    if (a.counts != nullptr && n != a.counts[e] && a.counts[e] > 0 && a.status != nullptr && blockIdx.x == 0)
+      atomicOr(a.status, FMOE_STATUS_BAD_EXPERT);  // rows past the end of A were cut off
+    chunk_prefix[e + 1] = static_cast<int>((n + kTokens - 1) / kTokens);
+  }
+  if (threadIdx.x == 0) chunk_prefix[0] = 0;
+  __syncthreads();
+  if (warp == 0) {
+    int carry = 0;
+    for (int base = 0; base < a.E; base += 32) {
+      const int e = base + lane;
+      int v = e < a.E ? chunk_prefix[e + 1] : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int n = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += n;
+      }
+      if (e < a.E) chunk_prefix[e + 1] = carry + v;
+      carry += __shfl_sync(0xffffffffu, v, 31);
+    }
+  }
+  __syncthreads();
+  const int items = chunk_prefix[a.E] * f.n_blocks;
+  const int out_cols = swiglu ? kFewRows / 2 : kFewRows;
+
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    int lo = 0, hi = a.E;  // last e with chunk_prefix[e] * n_blocks <= item
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (chunk_prefix[mid] * f.n_blocks <= item) lo = mid; else hi = mid;
+    }
+    const int chunks = chunk_prefix[lo + 1] - chunk_prefix[lo];
+    const int local = item - chunk_prefix[lo] * f.n_blocks;
+    const int nb = local / chunks, chunk = local - nb * chunks;  // chunks that share weights run together
+    const int64_t row0 = (a.offsets == nullptr ? 0 : a.offsets[lo]) + static_cast<int64_t>(chunk) * kTokens;
+    const int64_t left = rows_of(a, lo) - static_cast<int64_t>(chunk) * kTokens;
+    const int rows = static_cast<int>(left < kTokens ? left : kTokens);
+
+    // this lane's four weight rows: g and g + 8 of each 16-row operand; past the end the last row again
+    const int8_t* w_row[2][2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        int64_t n = swiglu ? static_cast<int64_t>(nb) * 16 + 8 * h + g : static_cast<int64_t>(nb) * kFewRows + 16 * m + 8 * h + g;
+        if (n >= a.cols) n = a.cols - 1;
+        if (swiglu) n += m * a.cols;
+        w_row[m][h] = f.W + lo * f.w_expert_stride + n * f.w_stride + 16 * t;
+      }
+    const int8_t* tok[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) tok[j] = 8 * j + g < rows ? f.A + (row0 + 8 * j + g) * f.a_stride : nullptr;
+
+    int acc[2][NT][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][j][i] = 0;
+
+    // One step ahead: the next step's weights and tokens are on their way while this one's are multiplied.
+    uint4 w[2][2][2], b[2][NT];  // weights [m][g or g + 8][64-byte half of the step]; tokens [half][j]
+    auto load = [&](int k) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const bool in = k + 64 * s + 16 * t < K;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            w[m][h][s] = in ? ld_stream16(reinterpret_cast<const uint4*>(w_row[m][h] + k + 64 * s)) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) b[s][j] = load_token(tok[j], k + 64 * s + 16 * t, K);
+    };
+    int k = warp * kFewStep;
+    if (k < K) load(k);
+    while (k < K) {
+      uint4 cw[2][2][2], cb[2][NT];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) cw[m][h][s] = w[m][h][s];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) cb[s][j] = b[s][j];
+      }
+      k += kFewWarps * kFewStep;
+      if (k < K) load(k);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+            mma_s8(acc[m][j], cw[m][0][s].x, cw[m][1][s].x, cw[m][0][s].y, cw[m][1][s].y, cb[s][j].x, cb[s][j].y);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+            mma_s8(acc[m][j], cw[m][0][s].z, cw[m][1][s].z, cw[m][0][s].w, cw[m][1][s].w, cb[s][j].z, cb[s][j].w);
+      }
+    }
+    __syncthreads();  // the previous item's sums have been read
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) red[warp][8 * j + 2 * t + (i & 1)][16 * m + g + 8 * (i >> 1)] = acc[m][j][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < kTokens * out_cols; i += kFewThreads) {
+      const int token = i / out_cols, c = i - token * out_cols;
+      const int64_t col = static_cast<int64_t>(nb) * out_cols + c;
+      if (token < rows && col < a.cols) {
+        int sum = 0, up = 0;
+#pragma unroll
+        for (int v = 0; v < kFewWarps; ++v) {
+          sum += red[v][token][c];
+          if (swiglu) up += red[v][token][16 + c];
+        }
+        const float sa = a.a_scale[row0 + token];
+        const float* sw = a.w_scale + static_cast<int64_t>(lo) * a.N;
+        float y = static_cast<float>(sum) * sa * sw[col];
+        if (swiglu) y = y * sigmoid(y) * (static_cast<float>(up) * sa * sw[a.cols + col]);
+        else if (a.act == FMOE_ACT_GELU) y = gelu(y);
+        static_cast<E*>(a.C)[(row0 + token) * a.cols + col] = from_float<DT>(y);
+      }
+    }
+  }
+}
+
+// ---- up to a few hundred rows: weight rows as the MMA's M, tokens as its N, K split over a cluster ----
+// A 128 x 256 tile streams 48 KB of operands per 128 bytes of K through one SM at 64 bytes a clock, and
+// with few tiles most SMs watch: 7168 x 7168 weights took 32 us for any number of rows up to 512. Here
+// the tile is 128 weight rows (64 gate + 64 up rows for SwiGLU) x NB tokens, so that for few tokens
+// nearly all of an SM's traffic is weights, two CTAs share an SM, and where even that leaves SMs idle
+// the K range is split over the S CTAs of a cluster. Their integer sums meet in distributed
+// shared memory: exact, whatever the split.
+// The accumulator arrives with lane = output column and column = token: a warp's stores of one token
+// are 32 consecutive columns as they come.
+constexpr int kTnRows = 128;
+constexpr int kTnWBytes = kTnRows * kBK;  // 16 KB
+template <int NB>
+struct Tn {
+  static constexpr int kStages = NB <= 32 ? 5 : NB <= 64 ? 4 : 3;  // two CTAs fit an SM
+  static constexpr int kStageBytes = kTnWBytes + NB * kBK;
+  static constexpr int kTmemCols = 2 * NB < 32 ? 32 : 2 * NB;  // two accumulators
+};
+constexpr int kTnExchange = 16 * 64;  // floats: up halves of 16 tokens on their way to the gate warps
+
+struct TnArgs {
+  Args g;
+  int n_blocks;  // tiles of 128 weight rows (64 output columns for SwiGLU) per expert
+  int splits;    // CTAs per cluster, each with its share of K; 1: a persistent grid
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Four integers at `saddr` of CTA `rank`'s shared memory. Not volatile: the loads of one output go out
+// together. (A volatile load per CTA and output, one after the other, cost 20 us at 128 tokens.)
+__device__ __forceinline__ int4 ld_cluster4(uint32_t saddr, uint32_t rank) {
+  uint32_t remote;
+  int4 v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(saddr), "r"(rank));
+  asm("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(remote) : "memory");
+  return v;
+}
+// Barrier of the four epilogue warps that also tells whether one of them gave up: a warp must not wait
+// here for one that has left.
+__device__ __forceinline__ bool epilogue_any(bool gave_up) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(gave_up))
+      : "memory");
+  return any != 0;
+}
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// Up to four neighbouring outputs.
+__device__ __forceinline__ void store4(void* C, int64_t i, int dt, const float* y, int n, bool whole) {
+  if (whole && n == 4) {
+    if (dt == FMOE_F32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(C) + i) = make_float4(y[0], y[1], y[2], y[3]);
+    } else if (dt == FMOE_BF16) {
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0], y[1]), hi = __floats2bfloat162_rn(y[2], y[3]);
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(C) + i) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    } else {
+      const __half2 lo = __floats2half2_rn(y[0], y[1]), hi = __floats2half2_rn(y[2], y[3]);
+      *reinterpret_cast<uint2*>(static_cast<__half*>(C) + i) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) store_scalar_from_float(C, i + j, dt, y[j]);
+  }
+}
+
+template <int NB>
+__global__ void __launch_bounds__(kThreads, 2)
+    int8_tn_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_w, const TnArgs f) {
+  constexpr int kS = Tn<NB>::kStages, kStage = Tn<NB>::kStageBytes, kTmemCols = Tn<NB>::kTmemCols;
+  constexpr uint32_t kIdescTn = (2u << 4) | (1u << 7) | (1u << 10) | ((NB >> 3) << 17) | ((kTnRows >> 4) << 24);
+  static_assert(kS * kStage >= NB * kTnRows * 4, "the partial sums take the place of the pipeline");
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kS * kStage);
+  uint64_t* empty = full + kS;
+  uint64_t* tmem_full = empty + kS;
+  uint64_t* tmem_empty = tmem_full + 2;
+  uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
+  int* abort_flag = reinterpret_cast<int*>(tmem_base_slot + 1);
+  uint64_t* drain = reinterpret_cast<uint64_t*>(abort_flag + 1);
+  float* exchange = reinterpret_cast<float*>(smem + kS * kStage + 256);
+  int* chunk_prefix = reinterpret_cast<int*>(exchange + kTnExchange);  // [E + 1]
+  int* part = reinterpret_cast<int*>(smem);                            // [NB][128], after the pipeline has drained
+
+  const Args& a = f.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool swiglu = a.act == FMOE_ACT_SWIGLU;
+  const int out_cols = swiglu ? kTnRows / 2 : kTnRows;
+  const int split = f.splits > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int k_begin = a.k_blocks * split / f.splits, k_end = a.k_blocks * (split + 1) / f.splits;
+  int fills = 0;
+  bool mma_issued = false;
+
+  // ---- set-up ----------------------------------------------------------------------------
+  for (int e = threadIdx.x; e < a.E; e += kThreads) {
+    const int64_t n = rows_of(a, e);
+    if (a.counts != nullptr && n != a.counts[e] && a.counts[e] > 0 && a.status != nullptr && blockIdx.x == 0)
+      atomicOr(a.status, FMOE_STATUS_BAD_EXPERT);  // rows past the end of A were cut off
+    chunk_prefix[e + 1] = static_cast<int>((n + NB - 1) / NB);
+  }
+  if (threadIdx.x == 0) {
+    chunk_prefix[0] = 0;
+    *abort_flag = 0;
+    for (int s = 0; s < kS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tmem_full[i], 1);
+      mbar_init(&tmem_empty[i], 4);
+    }
+    mbar_init(drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int carry = 0;
+    for (int base = 0; base < a.E; base += 32) {
+      const int e = base + lane;
+      int v = e < a.E ? chunk_prefix[e + 1] : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int n = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += n;
+      }
+      if (e < a.E) chunk_prefix[e + 1] = carry + v;
+      carry += __shfl_sync(0xffffffffu, v, 31);
+    }
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)),
+                 "n"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = *tmem_base_slot;
+  const int items = chunk_prefix[a.E] * f.n_blocks;
+  const int first = static_cast<int>(blockIdx.x) / f.splits, stride = static_cast<int>(gridDim.x) / f.splits;
+
+  struct Item {
+    int expert, nb, rows;
+    int64_t row0;
+  };
+  auto find = [&](int item) {  // the chunks of an expert's rows that read the same weights are neighbours
+    int lo = 0, hi = a.E;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (chunk_prefix[mid] * f.n_blocks <= item) lo = mid; else hi = mid;
+    }
+    const int chunks = chunk_prefix[lo + 1] - chunk_prefix[lo];
+    const int local = item - chunk_prefix[lo] * f.n_blocks;
+    Item t;
+    t.expert = lo;
+    t.nb = local / chunks;
+    const int64_t begin = static_cast<int64_t>(local - t.nb * chunks) * NB;
+    t.row0 = (a.offsets == nullptr ? 0 : a.offsets[lo]) + begin;
+    const int64_t rows = rows_of(a, lo) - begin;
+    t.rows = static_cast<int>(rows < NB ? rows : NB);
+    return t;
+  };
+
+  if (warp == 0 && lane == 0) {
+    // ---- TMA producer ---------------------------------------------------------------
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int item = first; item < items && !a.skip_loads; item += stride) {
+      const Item t = find(item);
+      for (int kb = k_begin; kb < k_end; ++kb) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, a.spin_limit)) goto timed_out;
+        mbar_expect_tx(&full[stage], kStage);
+        uint8_t* w = smem + stage * kStage;
+        if (swiglu) {  // 64 gate rows, then the up rows of the same columns
+          tma_load_3d(w, &map_w, kb * kBK, t.nb * 64, t.expert, &full[stage]);
+          tma_load_3d(w + kTnWBytes / 2, &map_w, kb * kBK, static_cast<int>(a.cols) + t.nb * 64, t.expert, &full[stage]);
+        } else {
+          tma_load_3d(w, &map_w, kb * kBK, t.nb * kTnRows, t.expert, &full[stage]);
+        }
+        tma_load_2d(w + kTnWBytes, &map_t, kb * kBK, static_cast<int>(t.row0), &full[stage]);
+        ++fills;
+        if (++stage == kS) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1 && lane == 0) {
+    // ---- MMA issuer -----------------------------------------------------------------
+    int stage = 0;
+    uint32_t phase = 0;
+    int it = 0;
+    for (int item = first; item < items; item += stride, ++it) {
+      const int acc = it & 1;
+      if (!mbar_wait(&tmem_empty[acc], ((it >> 1) & 1) ^ 1, abort_flag, a.spin_limit)) goto timed_out;
+      tcgen05_fence_after();
+      for (int kb = k_begin; kb < k_end; ++kb) {
+        if (!mbar_wait(&full[stage], phase, abort_flag, a.spin_limit)) goto timed_out;
+        tcgen05_fence_after();
+        mma_issued = true;
+        const uint64_t dw = smem_desc(smem_u32(smem + stage * kStage));
+        const uint64_t dt = smem_desc(smem_u32(smem + stage * kStage + kTnWBytes));
+#pragma unroll
+        for (int k = 0; k < kBK / kUmmaK; ++k)
+          umma_i8(tmem_base + acc * NB, dw + 2 * k, dt + 2 * k, kIdescTn, kb > k_begin || k > 0 ? 1u : 0u);
+        umma_commit(&empty[stage]);
+        if (++stage == kS) { stage = 0; phase ^= 1; }
+      }
+      umma_commit(&tmem_full[acc]);
+    }
+  } else if (warp >= 2) {
+    // ---- epilogue -------------------------------------------------------------------
+    const int quarter = warp & 3, line = quarter * 32 + lane;  // line: weight row of the tile
+    int it = 0;
+    for (int item = first; item < items; item += stride, ++it) {
+      const int acc = it & 1;
+      const Item t = find(item);
+      const int64_t col = static_cast<int64_t>(t.nb) * out_cols + (line & (out_cols - 1));
+      const bool up = swiglu && line >= 64;
+      const float sw = col < a.cols ? a.w_scale[static_cast<int64_t>(t.expert) * a.N + (up ? a.cols : 0) + col] : 0.f;
+      if (epilogue_any(!mbar_wait(&tmem_full[acc], (it >> 1) & 1, abort_flag, a.spin_limit))) goto timed_out;
+      tcgen05_fence_after();
+      const uint32_t taddr = tmem_base + acc * NB + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll 1
+      for (int c0 = 0; c0 < t.rows; c0 += 16) {
+        uint32_t r[16];
+        tmem_ld16(taddr + c0, r);
+        tmem_ld_wait();
+        if (f.splits > 1) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) part[(c0 + i) * kTnRows + line] = static_cast<int>(r[i]);
+          continue;
+        }
+        const float mine = c0 + (lane & 15) < t.rows ? a.a_scale[t.row0 + c0 + (lane & 15)] : 0.f;
+        float y[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[i] = static_cast<float>(static_cast<int>(r[i])) * __shfl_sync(0xffffffffu, mine, i) * sw;
+        if (swiglu) {
+          if (up) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) exchange[i * 64 + line - 64] = y[i];
+          }
+          epilogue_sync();
+          if (!up) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = y[i] * sigmoid(y[i]) * exchange[i * 64 + line];
+          }
+          epilogue_sync();
+        } else if (a.act == FMOE_ACT_GELU) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) y[i] = gelu(y[i]);
+        }
+        if (!up && col < a.cols) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (c0 + i < t.rows) store_scalar_from_float(a.C, (t.row0 + c0 + i) * a.cols + col, a.out_dtype, y[i]);
+        }
+      }
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tmem_empty[acc]);
+    }
+  }
+  goto done;
+
+timed_out:
+  *abort_flag = 1;
+  if (a.status != nullptr) atomicOr(a.status, FMOE_STATUS_WAIT_TIMEOUT);
+
+done:
+  drain_on_exit(warp, lane, fills, mma_issued, full, drain, abort_flag, kS, a.spin_limit);
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "n"(kTmemCols) : "memory");
+  }
+  if (f.splits == 1) return;
+  // One item per cluster: every CTA adds up its share of the outputs over the cluster's partial sums.
+  // All threads of all its CTAs come here, also after a wait gave up.
+  __syncwarp();
+  cluster_sync_all();
+  if (first < items) {
+    const Item t = find(first);
+    const uint32_t base = smem_u32(part);
+    const float* scales = a.w_scale + static_cast<int64_t>(t.expert) * a.N;
+    // four neighbouring columns of a token at a time
+    for (int i = split * kThreads + threadIdx.x; i < t.rows * (out_cols / 4); i += f.splits * kThreads) {
+      const int token = i / (out_cols / 4), c = (i - token * (out_cols / 4)) * 4;
+      const int64_t col = static_cast<int64_t>(t.nb) * out_cols + c;
+      if (col >= a.cols) continue;
+      const uint32_t at = base + 4 * (token * kTnRows + c);
+      int4 sum = make_int4(0, 0, 0, 0), up = sum;
+#pragma unroll 8
+      for (int r = 0; r < f.splits; ++r) {
+        const int4 v = ld_cluster4(at, r);
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+      }
+      if (swiglu) {
+#pragma unroll 8
+        for (int r = 0; r < f.splits; ++r) {
+          const int4 v = ld_cluster4(at + 4 * 64, r);
+          up.x += v.x, up.y += v.y, up.z += v.z, up.w += v.w;
+        }
+      }
+      const float sa = a.a_scale[t.row0 + token];
+      const int sums[4] = {sum.x, sum.y, sum.z, sum.w}, ups[4] = {up.x, up.y, up.z, up.w};
+      float y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t n = col + j < a.cols ? col + j : col;
+        y[j] = static_cast<float>(sums[j]) * sa * scales[n];
+        if (swiglu) y[j] = y[j] * sigmoid(y[j]) * (static_cast<float>(ups[j]) * sa * scales[a.cols + n]);
+        else if (a.act == FMOE_ACT_GELU) y[j] = gelu(y[j]);
+      }
+      store4(a.C, (t.row0 + token) * a.cols + col, a.out_dtype, y, static_cast<int>(a.cols - col < 4 ? a.cols - col : 4),
+             a.cols % 4 == 0 && a.vec_ok != 0);
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();  // no CTA leaves while another reads its sums
+}
+
 // int8 tensor [depth, rows, cols] with the given strides in bytes (depth 1: [rows, cols]), box =
 // 128 columns x box_rows rows, 128-byte swizzle; coordinates outside read as zeros.
 static int make_map(CUtensorMap* map, const void* base, int64_t depth, int64_t rows, int64_t cols, int64_t row_stride,
@@ -341,7 +870,43 @@ static int make_map(CUtensorMap* map, const void* base, int64_t depth, int64_t r
   return FMOE_OK;
 }
 
+template <int DT, int NT>
+static int launch_few(const FewArgs& f, int64_t items, cudaStream_t st) {
+  static_assert(sizeof(int) * kFewWarps * 8 * NT * (kFewRows + kFewPad) <= 40 * 1024, "static and dynamic part within 48 KB");
+  int per_sm = 0;
+  const int smem = static_cast<int>(sizeof(int)) * (f.g.E + 1);
+  FMOE_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, int8_few_rows_kernel<DT, NT>, kFewThreads, smem));
+  const int64_t most = static_cast<int64_t>(per_sm > 0 ? per_sm : 1) * kNumSMs;
+  int8_few_rows_kernel<DT, NT><<<static_cast<unsigned>(items < most ? items : most), kFewThreads, smem, st>>>(f);
+  return check_launch("int8_few_rows_kernel");
+}
+
+template <int NB>
+static int launch_tn(const CUtensorMap& map_t, const CUtensorMap& map_w, const TnArgs& f, int64_t items, cudaStream_t st) {
+  constexpr int kFixed = 1024 + Tn<NB>::kStages * Tn<NB>::kStageBytes + 256 + 4 * kTnExchange;
+  const size_t smem = kFixed + sizeof(int) * (f.g.E + 2);
+  FMOE_CUDA(cudaFuncSetAttribute(int8_tn_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kFixed + static_cast<int>(sizeof(int)) * (kMaxExperts + 2)));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  const int64_t most = 2 * static_cast<int64_t>(g_gemm_sms);
+  cfg.gridDim = dim3(static_cast<unsigned>(f.splits > 1 ? items * f.splits : items < most ? items : most));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = f.splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = f.splits > 1 ? 1 : 0;
+  FMOE_CUDA(cudaLaunchKernelEx(&cfg, int8_tn_kernel<NB>, map_t, map_w, f));
+  return check_launch("int8_tn_kernel");
+}
+
 }  // namespace i8
+
+int g_int8_few_rows = -1;  // fmoe_tune "int8_few_rows": 1 / 0 forces the kernel, -1 = by the sizes
+
 }  // namespace fmoe
 
 using namespace fmoe;
@@ -388,6 +953,56 @@ extern "C" int fmoe_int8_gemm(const int8_t* a, int64_t a_stride, const float* a_
   g.spin_limit = static_cast<uint32_t>(g_gemm_spin_limit);
   g.status = status;
   FMOE_REQUIRE((R / i8::kBM + E) * g.n_blocks < (1ll << 31), FMOE_ERR_UNSUPPORTED, "fmoe_int8_gemm: too many tiles");
+  // Which kernel: the host knows the rows and the experts, not how the rows are spread.
+  const int64_t mean = (R + E - 1) / E, touched = (R < E ? R : E) * N * K;
+  const int64_t tokens = E == 1 ? R : 2 * mean;  // rows that an expert may well have
+  int which = g_int8_few_rows;
+  if (which < 0) {
+    const int64_t tiles = ((R + i8::kBM - 1) / i8::kBM + (R < E ? R : E) - 1) * g.n_blocks;
+    // One pass over the weights for every eight rows of an expert costs the few-rows kernel 2 us per 16 MB
+    // after a start of 3 us; the split-K kernel starts at 5 to 6 us and the tiled one at 8 to 9 us. Measured
+    // (few / split K / tiled, us): 512 x 4096, 8 rows 3.4 / 5.8 / 8.8, 64 rows 7.9 / 9.1 / 9.2; 2048 x 7168, 8
+    // rows 6.6 / 8.9 / 16.6, 24 rows 11.3 / 9.5 / 17.0. A tile of the tiled kernel takes the same time for 1 row
+    // and for 128, so it needs tiles for most SMs: 7168 x 7168, 256 rows (56 tiles) - / 26 / 33, 512 rows
+    // (112) - / 35 / 32; 64 experts of 7168 x 4096, 32 rows each - / 282 / 292, 128 each - / 359 / 339.
+    which = tokens <= i8::kFewTokens && (tokens + 7) / 8 * touched <= i8::kFewBytes ? 1 : mean <= 64 || tiles <= 56 ? 2 : 0;
+  }
+  if (which == 1) {
+    i8::FewArgs f;
+    f.A = a;
+    f.W = w;
+    f.a_stride = a_stride;
+    f.w_stride = w_stride;
+    f.w_expert_stride = E == 1 ? 0 : w_expert_stride;
+    f.K = K;
+    f.n_blocks = static_cast<int>(swiglu ? (cols + 15) / 16 : (N + i8::kFewRows - 1) / i8::kFewRows);
+    f.g = g;
+    const int64_t items = (R / 8 + (R < E ? R : E)) * f.n_blocks;
+    FMOE_REQUIRE(items < (1ll << 31), FMOE_ERR_UNSUPPORTED, "fmoe_int8_gemm: too many tiles");
+    int rc = FMOE_OK;
+    FMOE_DISPATCH_DTYPE(out_dtype, DT, rc = (i8::launch_few<DT, 1>(f, items, static_cast<cudaStream_t>(stream))));
+    return rc;
+  }
+  if (which == 2) {
+    i8::TnArgs f;
+    f.g = g;
+    f.n_blocks = static_cast<int>(swiglu ? (cols + 63) / 64 : (N + i8::kTnRows - 1) / i8::kTnRows);
+    const int nb = tokens <= 16 ? 16 : tokens <= 32 ? 32 : tokens <= 64 ? 64 : 128;
+    const int64_t items = (E == 1 ? (R + nb - 1) / nb : R / nb + (R < E ? R : E)) * f.n_blocks;
+    FMOE_REQUIRE(items < (1ll << 31) / 8, FMOE_ERR_UNSUPPORTED, "fmoe_int8_gemm: too many tiles");
+    f.splits = 1;
+    while (f.splits < 8 && items * f.splits * 2 <= 2 * kNumSMs && g.k_blocks / (f.splits * 2) >= 2) f.splits *= 2;
+    CUtensorMap map_t, map_w;
+    int rc = i8::make_map(&map_t, a, 1, R, K, a_stride, R * a_stride, nb, 2, "A");
+    if (rc != 0) return rc;
+    rc = i8::make_map(&map_w, w, E, N, K, w_stride, E == 1 ? N * w_stride : w_expert_stride, swiglu ? 64 : i8::kTnRows, 3, "W");
+    if (rc != 0) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (nb == 16) return i8::launch_tn<16>(map_t, map_w, f, items, st);
+    if (nb == 32) return i8::launch_tn<32>(map_t, map_w, f, items, st);
+    if (nb == 64) return i8::launch_tn<64>(map_t, map_w, f, items, st);
+    return i8::launch_tn<128>(map_t, map_w, f, items, st);
+  }
   CUtensorMap map_a, map_w;
   int rc = i8::make_map(&map_a, a, 1, R, K, a_stride, R * a_stride, i8::kBM, 2, "A");
   if (rc != 0) return rc;
@@ -401,7 +1016,7 @@ extern "C" int fmoe_int8_gemm(const int8_t* a, int64_t a_stride, const float* a_
                         static_cast<int>(sizeof(int)) * (i8::kMaxExperts + 2);
   FMOE_DISPATCH_DTYPE(out_dtype, DT, {
     FMOE_CUDA(cudaFuncSetAttribute(i8::int8_gemm_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_most));
-    i8::int8_gemm_kernel<DT><<<grid, i8::kThreads, smem, static_cast<cudaStream_t>(stream)>>>(map_a, map_w, g);
+    i8::int8_gemm_kernel<DT><<<grid, i8::kTileThreads, smem, static_cast<cudaStream_t>(stream)>>>(map_a, map_w, g);
   });
   return check_launch("int8_gemm_kernel");
 }

@@ -16,7 +16,7 @@ constexpr int kGroup = 128;
 
 // f[0..8) of a row from column c on (zeros past D).
 template <int DT>
-__device__ __forceinline__ void load8(const void* row, int64_t c, int64_t D, int vec, float* f) {
+__device__ __forceinline__ void load8(const void* row, int c, int D, int vec, float* f) {
   using E = typename Elem<DT>::type;
   const E* p = static_cast<const E*>(row) + c;
   if (vec) {
@@ -28,7 +28,7 @@ __device__ __forceinline__ void load8(const void* row, int64_t c, int64_t D, int
   }
 }
 template <int DT>
-__device__ __forceinline__ void store8(void* row, int64_t c, int64_t D, int vec, const float* f) {
+__device__ __forceinline__ void store8(void* row, int c, int D, int vec, const float* f) {
   using E = typename Elem<DT>::type;
   E* p = static_cast<E*>(row) + c;
   if (vec) {
@@ -42,30 +42,47 @@ __device__ __forceinline__ void store8(void* row, int64_t c, int64_t D, int vec,
 }
 // Eight packed values from column c on, as floats; rows of q lie at 16-byte steps with zeros up to
 // the next step, so eight bytes from a multiple of eight are always there.
-__device__ __forceinline__ void load8_packed(const int8_t* row, int64_t c, float s, float* f) {
-  const uint2 w = *reinterpret_cast<const uint2*>(row + c);
-  unpack_int8(w.x, f);
-  unpack_int8(w.y, f + 4);
+__device__ __forceinline__ void dequantise8(uint2 w, float s, float2* f) {
+  const float2 s2 = make_float2(s, s);
+  float t[8];
+  unpack_int8(w.x, t);
+  unpack_int8(w.y, t + 4);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] *= s;
+  for (int j = 0; j < 4; ++j) f[j] = mul2(make_float2(t[2 * j], t[2 * j + 1]), s2);
 }
+
+// Quotients by a run-time constant, as a multiplication: n / d = n * (2^s / d + 1) / 2^s for n < 2^31,
+// with s = 31 + ceil(log2 d) (the excess of the factor, below 2^-s each, adds less than 1 / d).
+struct FastDiv {
+  uint32_t mul = 0, shift = 0;
+  int d = 1;
+  explicit FastDiv(int64_t divisor) : d(static_cast<int>(divisor)) {
+    uint32_t log = 0;
+    while ((1ll << log) < divisor) ++log;
+    shift = 31 + log;
+    mul = static_cast<uint32_t>((1ull << shift) / static_cast<uint64_t>(divisor) + 1);
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul) >> shift);
+  }
+};
 
 // Eight lanes share a group, sixteen columns each.
 template <int DT>
 __global__ void __launch_bounds__(256) pack_kernel(const void* x, int64_t x_stride, int8_t* q, int64_t q_stride,
-                                                   float* scale, int64_t T, int64_t D, int groups, int vec) {
+                                                   float* scale, int total, int D, FastDiv groups, int vec) {
   using E = typename Elem<DT>::type;
   constexpr int VE = Elem<DT>::kVec;
-  const int64_t total = T * groups;
   const int sub = threadIdx.x & 7;
   // the four groups of a warp stay in the loop together: the shuffles below need all 32 lanes
   for (int64_t g0 = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x >> 5) * 4; g0 < total;
        g0 += static_cast<int64_t>(gridDim.x) * 32) {
-    const int64_t g = g0 + ((threadIdx.x >> 3) & 3);
+    const int g = static_cast<int>(g0) + ((threadIdx.x >> 3) & 3);
     const bool live = g < total;
-    const int64_t row = live ? g / groups : 0;
-    const int k = static_cast<int>(g - row * groups);
-    const int64_t c = static_cast<int64_t>(k) * kGroup + sub * 16;
+    const int row_of = live ? groups.div(g) : 0;
+    const int64_t row = row_of;
+    const int k = g - row_of * groups.d;
+    const int c = k * kGroup + sub * 16;
     const E* p = static_cast<const E*>(x) + row * x_stride + c;
     uint4 v[16 / VE];
     uint32_t top = 0;
@@ -96,82 +113,90 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* x, int64_t x_stri
       quant.operator()<16>(f, w);
       st_stream16(reinterpret_cast<uint4*>(q + row * q_stride + c), make_uint4(w[0], w[1], w[2], w[3]));
     }
-    if (live && sub == 0) scale[row * groups + k] = quant.scale;
+    if (live && sub == 0) scale[g] = quant.scale;
   }
 }
 
 template <int DT>
 __global__ void __launch_bounds__(256) unpack_kernel(const int8_t* q, int64_t q_stride, const float* scale, void* out,
-                                                     int64_t T, int64_t D, int groups, int vec) {
+                                                     int total, int D, int groups, FastDiv per_row, int vec) {
   using E = typename Elem<DT>::type;
-  const int64_t per_row = (D + 7) / 8, total = T * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t row = i / per_row, c = (i - row * per_row) * 8;
-    float f[8];
-    load8_packed(q + row * q_stride, c, scale[row * groups + c / kGroup], f);
-    store8<DT>(static_cast<E*>(out) + row * D, c, D, vec, f);
+    const int row_of = per_row.div(static_cast<int>(i)), c = (static_cast<int>(i) - row_of * per_row.d) * 8;
+    const int64_t row = row_of;
+    float2 f[4];
+    dequantise8(*reinterpret_cast<const uint2*>(q + row * q_stride + c), scale[row * groups + c / kGroup], f);
+    store8<DT>(static_cast<E*>(out) + row * D, c, D, vec, reinterpret_cast<const float*>(f));
   }
 }
 
-// The fast exponential and quotient are off by (2 + |x|) and 2 steps of 2^-23: the result goes into
-// products that are rounded to 16 bits, or held to a 32-bit bound that counts them.
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
-
-// One thread: eight columns of the gate half and the same columns of the up half. A width that is
-// not a multiple of eight leaves the up half's bytes off the 8-byte grid: they are read one by one.
+// One thread: eight columns of the gate half and the same columns of the up half. A width that is not a multiple of eight leaves the up half's bytes off the 8-byte grid: they are read
+// one by one.
 template <int DT>
 __global__ void __launch_bounds__(256) packed_swiglu_bwd_kernel(const int8_t* q, int64_t q_stride, const float* scale,
                                                                 const void* grad, int64_t g_stride, void* grad_h,
-                                                                void* hidden, int64_t T, int64_t ff, int groups, int vec) {
+                                                                void* hidden, int total, int ff, int groups,
+                                                                FastDiv per_row, int vec) {
   using E = typename Elem<DT>::type;
-  const int64_t per_row = (ff + 7) / 8, total = T * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t row = i / per_row, c = (i - row * per_row) * 8;
+    const int row_of = per_row.div(static_cast<int>(i)), c = (static_cast<int>(i) - row_of * per_row.d) * 8;
+    const int64_t row = row_of;
     const int8_t* qr = q + row * q_stride;
     const float* sr = scale + row * groups;
-    float gate[8], up[8], g[8], d[8], h[8];
-    load8<DT>(static_cast<const E*>(grad) + row * g_stride, c, ff, vec, g);
-    load8_packed(qr, c, sr[c / kGroup], gate);
+    float2 gate[4], up[4], g[4], d[4], h[4];
+    const uint2 qg = *reinterpret_cast<const uint2*>(qr + c);
     if (vec) {
-      load8_packed(qr, ff + c, sr[(ff + c) / kGroup], up);
+      const uint2 qu = *reinterpret_cast<const uint2*>(qr + ff + c);
+      load8<DT>(static_cast<const E*>(grad) + row * g_stride, c, ff, 1, reinterpret_cast<float*>(g));
+      dequantise8(qu, sr[(ff + c) / kGroup], up);
     } else {
+      load8<DT>(static_cast<const E*>(grad) + row * g_stride, c, ff, 0, reinterpret_cast<float*>(g));
+      float* u = reinterpret_cast<float*>(up);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        up[j] = c + j < ff ? static_cast<float>(qr[ff + c + j]) * sr[(ff + c + j) / kGroup] : 0.f;
+        u[j] = c + j < ff ? static_cast<float>(qr[ff + c + j]) * sr[(ff + c + j) / kGroup] : 0.f;
     }
+    dequantise8(qg, sr[c / kGroup], gate);
+    const float2 one = make_float2(1.f, 1.f), minus = make_float2(-1.f, -1.f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float s = sigmoid(gate[j]), act = gate[j] * s;
-      h[j] = act * up[j];
-      d[j] = g[j] * up[j] * s * (1.f + gate[j] * (1.f - s));
-      up[j] = g[j] * act;
+    for (int j = 0; j < 4; ++j) {
+      const float2 s = make_float2(sigmoid(gate[j].x), sigmoid(gate[j].y));
+      const float2 act = mul2(gate[j], s);
+      h[j] = mul2(act, up[j]);
+      // d gate = grad up s (1 + gate (1 - s)),  d up = grad gate s
+      d[j] = mul2(mul2(mul2(g[j], up[j]), s), fma2(gate[j], fma2(s, minus, one), one));
+      up[j] = mul2(g[j], act);
     }
     E* out = static_cast<E*>(grad_h) + row * 2 * ff;
-    store8<DT>(out, c, ff, vec, d);
-    store8<DT>(out + ff, c, ff, vec, up);
-    store8<DT>(static_cast<E*>(hidden) + row * ff, c, ff, vec, h);
+    store8<DT>(out, c, ff, vec, reinterpret_cast<const float*>(d));
+    store8<DT>(out + ff, c, ff, vec, reinterpret_cast<const float*>(up));
+    store8<DT>(static_cast<E*>(hidden) + row * ff, c, ff, vec, reinterpret_cast<const float*>(h));
   }
 }
 
 template <int DT>
 __global__ void __launch_bounds__(256) packed_gelu_bwd_kernel(const int8_t* q, int64_t q_stride, const float* scale,
                                                               const void* grad, int64_t g_stride, void* grad_h,
-                                                              void* hidden, int64_t T, int64_t D, int groups, int vec) {
+                                                              void* hidden, int total, int D, int groups,
+                                                              FastDiv per_row, int vec) {
   using E = typename Elem<DT>::type;
-  const int64_t per_row = (D + 7) / 8, total = T * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t row = i / per_row, c = (i - row * per_row) * 8;
-    float x[8], g[8], h[8];
+    const int row_of = per_row.div(static_cast<int>(i)), c = (static_cast<int>(i) - row_of * per_row.d) * 8;
+    const int64_t row = row_of;
+    float2 x2[4];
+    float g[8], h[8];
     load8<DT>(static_cast<const E*>(grad) + row * g_stride, c, D, vec, g);
-    load8_packed(q + row * q_stride, c, scale[row * groups + c / kGroup], x);
+    dequantise8(*reinterpret_cast<const uint2*>(q + row * q_stride + c), scale[row * groups + c / kGroup], x2);
+    const float* x = reinterpret_cast<const float*>(x2);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float cdf = 0.5f * (1.f + erff(x[j] * 0.70710678118654752f));
+      float bell;
+      const float cdf = normal_cdf(x[j], &bell);
       h[j] = x[j] * cdf;
-      g[j] *= cdf + x[j] * 0.39894228040143268f * __expf(-0.5f * x[j] * x[j]);  // 1 / sqrt(2 pi)
+      g[j] *= cdf + x[j] * 0.39894228040143268f * bell;  // 1 / sqrt(2 pi)
     }
     store8<DT>(static_cast<E*>(grad_h) + row * D, c, D, vec, g);
     store8<DT>(static_cast<E*>(hidden) + row * D, c, D, vec, h);
@@ -192,6 +217,7 @@ using namespace fmoe;
   FMOE_REQUIRE(valid_dtype(dtype), FMOE_ERR_ARG, name ": bad dtype");                                       \
   FMOE_REQUIRE(T >= 0 && D > 0 && T < (1ll << 31) && D < (1ll << 31), FMOE_ERR_ARG, name ": bad sizes");     \
   if (T == 0) return FMOE_OK;                                                                               \
+  FMOE_REQUIRE(T * ((D + 7) / 8) < (1ll << 31) - 1024, FMOE_ERR_UNSUPPORTED, name ": too many values");    \
   FMOE_REQUIRE(q && scale, FMOE_ERR_ARG, name ": null pointer argument");                                   \
   FMOE_REQUIRE(q_stride % 16 == 0 && q_stride >= D && q_stride < D + 16 && aligned_to(q, 16), FMOE_ERR_ARG, \
                name ": packed rows lie at 16-byte steps, the next one after D bytes")
@@ -205,8 +231,8 @@ extern "C" int fmoe_pack_activation(const void* x, int64_t x_stride, int8_t* q, 
   const int groups = packed_groups(D);
   const int vec = D % 8 == 0 && aligned_to(x, 16) && x_stride * dtype_size(dtype) % 16 == 0;
   FMOE_DISPATCH_DTYPE(dtype, DT, pack_kernel<DT><<<stream_grid((T * groups + 31) / 32), 256, 0,
-                                                   static_cast<cudaStream_t>(stream)>>>(x, x_stride, q, q_stride, scale, T,
-                                                                                        D, groups, vec));
+                                                   static_cast<cudaStream_t>(stream)>>>(x, x_stride, q, q_stride, scale,
+                                                                                        static_cast<int>(T * groups), static_cast<int>(D), FastDiv(groups), vec));
   return check_launch("pack_kernel");
 }
 
@@ -217,8 +243,8 @@ extern "C" int fmoe_unpack_activation(const int8_t* q, int64_t q_stride, const f
   FMOE_REQUIRE(out != nullptr, FMOE_ERR_ARG, "fmoe_unpack_activation: null pointer argument");
   const int vec = D % 8 == 0 && aligned_to(out, 16);
   FMOE_DISPATCH_DTYPE(dtype, DT, unpack_kernel<DT><<<stream_grid((T * ((D + 7) / 8) + 255) / 256), 256, 0,
-                                                     static_cast<cudaStream_t>(stream)>>>(q, q_stride, scale, out, T, D,
-                                                                                          packed_groups(D), vec));
+                                                     static_cast<cudaStream_t>(stream)>>>(
+      q, q_stride, scale, out, static_cast<int>(T * ((D + 7) / 8)), static_cast<int>(D), packed_groups(D), FastDiv((D + 7) / 8), vec));
   return check_launch("unpack_kernel");
 }
 
@@ -236,15 +262,19 @@ extern "C" int fmoe_packed_act_bwd(const int8_t* q, int64_t q_stride, const floa
   FMOE_REQUIRE(T == 1 || g_stride >= cols, FMOE_ERR_ARG, "fmoe_packed_act_bwd: grad's row stride is too small");
   const int vec = cols % 8 == 0 && aligned_to(grad, 16) && g_stride * dtype_size(dtype) % 16 == 0 && aligned_to(grad_h, 16) &&
                   aligned_to(hidden, 16);
-  const unsigned grid = stream_grid((T * ((cols + 7) / 8) + 255) / 256);
+  const int total = static_cast<int>(T * ((cols + 7) / 8));
+  const FastDiv per_row((cols + 7) / 8);
+  const unsigned grid = stream_grid((static_cast<int64_t>(total) + 255) / 256);
   const int groups = packed_groups(D);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (swiglu) {
     FMOE_DISPATCH_DTYPE(dtype, DT, packed_swiglu_bwd_kernel<DT><<<grid, 256, 0, st>>>(q, q_stride, scale, grad, g_stride,
-                                                                                    grad_h, hidden, T, cols, groups, vec));
+                                                                                    grad_h, hidden, total, static_cast<int>(cols), groups,
+                                                                                    per_row, vec));
   } else {
     FMOE_DISPATCH_DTYPE(dtype, DT, packed_gelu_bwd_kernel<DT><<<grid, 256, 0, st>>>(q, q_stride, scale, grad, g_stride,
-                                                                                  grad_h, hidden, T, cols, groups, vec));
+                                                                                  grad_h, hidden, total, static_cast<int>(cols), groups,
+                                                                                    per_row, vec));
   }
   return check_launch("packed_act_bwd_kernel");
 }
