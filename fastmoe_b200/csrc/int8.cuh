@@ -22,7 +22,7 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v
 // two's complement in the low bits of the sum. Conversion instructions run at an eighth of the rate of
 // an addition, too few for the values that HBM delivers.
 constexpr float kRounder = 12582912.f;  // 1.5 * 2^23
-constexpr float kNear = 0.5f - 3e-5f;
+constexpr float kNear = 0.5f - 5e-5f;
 
 // The fast exponential and quotient are off by (2 + |x|) and 2 steps of 2^-23. The exact quotient's
 // slow path is a branch per value, which keeps a lane's values from overlapping: with it the SwiGLU
@@ -79,14 +79,30 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 
 struct Quantiser {
   float top;    // a
-  float inv;    // 127 / a
+  float inv;    // 127 / a, off by two steps of 2^-23 or less
   float scale;  // a / 127, or NaN
   bool fine;
   __device__ explicit Quantiser(uint32_t top_bits) {
     fine = top_bits < kInfBits;
     top = fine ? fmaxf(__uint_as_float(top_bits), 0x1p-100f) : 1.f;
-    inv = __fdiv_rn(127.f, top);
+    inv = __fdividef(127.f * 0x1p-8f, top * 0x1p-8f);  // scaled: the fast quotient gives up above 2^126
     scale = fine ? __fdiv_rn(top, 127.f) : __uint_as_float(0x7fc00000u);
+  }
+  // v * inv is off by at most 127 * 2 * 2^-23 = 3.1e-5. A quotient that lies that close to the border
+  // between two whole numbers is compared with the border exactly. (One in 10000 of arbitrary values
+  // does; among 16-bit values one that is exactly a / 2, at 63.5, is common.)
+  __device__ __forceinline__ void settle(float v, float& s) const {
+    const float r = s - kRounder, d = fmaf(v, inv, -r);
+    if (fabsf(d) > kNear) {
+      // The border next to r on d's side is m / 2 with m = 2 r +- 1; the side of v is the sign of
+      // 254 v - m a, both taken times 2^-8 against overflow. m a = h + low exactly; 254 v - h and the
+      // difference that is left have 18 bits or fewer in units of v's last one: exact too.
+      const float sign = copysignf(1.f, d);
+      const float m = fmaf(2.f, r, sign) * 0x1p-8f;
+      const float h = m * top, low = fmaf(m, top, -h);
+      const float side = (fmaf(v, 254.f / 256.f, -h) - low) * sign;
+      if (side > 0.f || (side == 0.f && (__float_as_uint(s) & 1u))) s += sign;
+    }
   }
   // N values: words[i] holds q of v[4 i .. 4 i + 3] (N = 1: of v[0], in the low byte). The budget is
   // tight: three bytes of DRAM traffic per 16-bit value leave eight instructions for it, so the
@@ -94,39 +110,33 @@ struct Quantiser {
   template <int N>
   __device__ __forceinline__ void operator()(const float* v, uint32_t* words) const {
     float s[N];
-    float off = 0.f;  // largest distance between a quotient and the whole number it went to
     if constexpr (N == 1) {
       s[0] = fmaf(v[0], inv, kRounder);
-      off = fabsf(fmaf(v[0], inv, -(s[0] - kRounder)));
+      settle(v[0], s[0]);
     } else {
-      const float2 inv2 = make_float2(inv, inv), up = make_float2(kRounder, kRounder);
-      const float2 down = make_float2(-kRounder, -kRounder), minus = make_float2(-1.f, -1.f);
+      const float2 inv2 = make_float2(inv, inv), up = make_float2(kRounder, kRounder), minus = make_float2(-1.f, -1.f);
+      constexpr int kPart = N > 8 ? 4 : N;  // values that are looked at together
+      float off[N / kPart];                 // their largest distance between a quotient and the whole number it went to
 #pragma unroll
       for (int j = 0; j < N; j += 2) {
         const float2 x = make_float2(v[j], v[j + 1]);
         const float2 t = fma2(x, inv2, up);
-        const float2 d = fma2(x, inv2, mul2(add2(t, down), minus));
+        const float2 d = fma2(x, inv2, fma2(t, minus, up));
         s[j] = t.x;
         s[j + 1] = t.y;
-        off = fmaxf(off, fmaxf(fabsf(d.x), fabsf(d.y)));
+        const float most = fmaxf(fabsf(d.x), fabsf(d.y));
+        off[j / kPart] = j % kPart == 0 ? most : fmaxf(off[j / kPart], most);
       }
-    }
-    // v * (127 / a) is off by at most 127 * 2 * 2^-24 = 1.6e-5. A quotient that lies that close to the
-    // border between two whole numbers is compared with the border exactly. (One in 16000 of
-    // arbitrary values does; among 16-bit values one that is exactly a / 2, at 63.5, is common.)
-    if (off > kNear) {
+      float most = off[0];
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float r = s[j] - kRounder, d = fmaf(v[j], inv, -r);
-        if (fabsf(d) > kNear) {
-          // The border next to r on d's side is m / 2 with m = 2 r +- 1; the side of v is the sign of
-          // 254 v - m a, both taken times 2^-8 against overflow. m a = h + low exactly; 254 v - h and
-          // the difference that is left have 18 bits or fewer in units of v's last one: exact too.
-          const float sign = copysignf(1.f, d);
-          const float m = fmaf(2.f, r, sign) * 0x1p-8f;
-          const float h = m * top, low = fmaf(m, top, -h);
-          const float side = (fmaf(v[j], 254.f / 256.f, -h) - low) * sign;
-          if (side > 0.f || (side == 0.f && (__float_as_uint(s[j]) & 1u))) s[j] += sign;
+      for (int j = kPart; j < N; j += kPart) most = fmaxf(most, off[j / kPart]);
+      if (most > kNear) {
+#pragma unroll
+        for (int j = 0; j < N; j += kPart) {
+          if (kPart == N || off[j / kPart] > kNear) {
+#pragma unroll
+            for (int i = 0; i < kPart; ++i) settle(v[j + i], s[j + i]);
+          }
         }
       }
     }
