@@ -80,14 +80,14 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 struct Quantiser {
   float top;    // a
   float inv;    // 127 / a, off by two steps of 2^-23 or less
-  float scale;  // a / 127, or NaN
   bool fine;
   __device__ explicit Quantiser(uint32_t top_bits) {
     fine = top_bits < kInfBits;
     top = fine ? fmaxf(__uint_as_float(top_bits), 0x1p-100f) : 1.f;
     inv = __fdividef(127.f * 0x1p-8f, top * 0x1p-8f);  // scaled: the fast quotient gives up above 2^126
-    scale = fine ? __fdiv_rn(top, 127.f) : __uint_as_float(0x7fc00000u);
   }
+  // a / 127, or NaN: rounded as a quotient, for the one thread that stores it
+  __device__ __forceinline__ float scale() const { return fine ? __fdiv_rn(top, 127.f) : __uint_as_float(0x7fc00000u); }
   // v * inv is off by at most 127 * 2 * 2^-23 = 3.1e-5. A quotient that lies that close to the border
   // between two whole numbers is compared with the border exactly. (One in 10000 of arbitrary values
   // does; among 16-bit values one that is exactly a / 2, at 63.5, is common.)

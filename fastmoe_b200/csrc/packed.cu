@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* x, int64_t x_stri
       quant.operator()<16>(f, w);
       st_stream16(reinterpret_cast<uint4*>(q + row * q_stride + c), make_uint4(w[0], w[1], w[2], w[3]));
     }
-    if (live && sub == 0) scale[g] = quant.scale;
+    if (live && sub == 0) scale[g] = quant.scale();
   }
 }
 

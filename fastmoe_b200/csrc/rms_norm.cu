@@ -26,7 +26,7 @@ struct RowArgs {
   float* q_scale;
   int64_t T, D;
   int64_t x_stride, r_stride, q_stride;
-  double eps;
+  double eps, inv_d;  // inv_d: 1 / D
   int w_f32;
   int shift0, shift_step;  // see row_shift
 };
@@ -214,8 +214,15 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* part) {
   return v;
 }
 
-__device__ __forceinline__ float inv_rms(double sum_sq, int64_t D, double eps) {
-  return static_cast<float>(1.0 / sqrt(sum_sq / static_cast<double>(D) + eps));
+// 1 / sqrt(mean + eps) to the last bit of 64: the fp32 instruction's 22 good bits, doubled once by
+// Householder's iteration of third order. Quotient and root in 64 bits cost 150 instructions, which
+// every warp of a row would issue.
+__device__ __forceinline__ float inv_rms(double sum_sq, double inv_d, double eps) {
+  const double v = fma(sum_sq, inv_d, eps);
+  if (!(v > 1e-30 && v < 1e30)) return static_cast<float>(1.0 / sqrt(v));
+  const double y = static_cast<double>(rsqrtf(static_cast<float>(v)));
+  const double e = fma(-(v * y), y, 1.0);
+  return static_cast<float>(fma(y * e, fma(e, 0.375, 0.5), y));
 }
 
 // Threads that a CTA of these kernels may have: 16 elements a thread and more need over 64 registers.
@@ -256,8 +263,11 @@ __global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::k
     if constexpr (CUT == kShifted) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        sv[i].mask(first + i * step, span);
-        if (NORM && a.residual != nullptr) rv[i].mask(first + i * step, span);
+        const int e = first + i * step;
+        if (e < D) {
+          sv[i].mask(e, span);
+          if (NORM && a.residual != nullptr) rv[i].mask(e, span);
+        }
       }
     }
     if (NORM && a.residual != nullptr) {
@@ -287,7 +297,7 @@ __global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::k
 #pragma unroll
       for (int j = 0; j < VE; ++j) sq = fma(static_cast<double>(f[j]), static_cast<double>(f[j]), sq);
     }
-    rstd = inv_rms(row_sum<WARP>(sq, part_sum), a.D, a.eps);
+    rstd = inv_rms(row_sum<WARP>(sq, part_sum), a.inv_d, a.eps);
     if (a.rstd != nullptr && tid == 0) a.rstd[row] = rstd;
   }
   auto value = [&](int i, float* f) {
@@ -335,7 +345,7 @@ __global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::k
   }
   const int pad = static_cast<int>((16 - (a.D & 15)) & 15);  // up to the next 16 bytes: zeros
   if (tid < pad) q[a.D + tid] = 0;
-  if (tid == 0) a.q_scale[row] = quant.scale;
+  if (tid == 0) a.q_scale[row] = quant.scale();
 }
 
 // Rows too wide for registers: three passes over the row, the later ones out of L2.
@@ -360,7 +370,7 @@ __global__ void __launch_bounds__(1024) row_loop_kernel(const RowArgs a) {
   }
   float rstd = 1.f;
   if constexpr (NORM) {
-    rstd = inv_rms(row_sum<false>(sq, part_sum), a.D, a.eps);
+    rstd = inv_rms(row_sum<false>(sq, part_sum), a.inv_d, a.eps);
     if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = rstd;
   }
   auto value = [&](int c) {
@@ -389,7 +399,7 @@ __global__ void __launch_bounds__(1024) row_loop_kernel(const RowArgs a) {
   }
   const int pad = static_cast<int>((16 - (a.D & 15)) & 15);
   if (threadIdx.x < pad) q[a.D + threadIdx.x] = 0;
-  if (threadIdx.x == 0) a.q_scale[row] = quant.scale;
+  if (threadIdx.x == 0) a.q_scale[row] = quant.scale();
 }
 
 // ---- backward -------------------------------------------------------------------------------
@@ -403,6 +413,7 @@ struct RowBwdArgs {
   float* part;  // optional [gridDim.x, D]: this CTA's share of dw
   int64_t T, D;
   int64_t dy_stride, ds_stride, s_stride;
+  float inv_d;  // 1 / D
   int w_f32;
   int shift0, shift_step;
 };
@@ -513,8 +524,11 @@ __global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::k
     if constexpr (CUT == kShifted) {  // what lies outside the row counts as zero; ds only meets the store
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        sv[i].mask(first + i * step, span);
-        gv[i].mask(first + i * step, span);
+        const int e = first + i * step;
+        if (e < D) {
+          sv[i].mask(e, span);
+          gv[i].mask(e, span);
+        }
       }
     }
     float dot = 0.f;
@@ -533,7 +547,7 @@ __global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::k
         }
       }
     }
-    const float mean = row_sum<WARP>(dot, part_sum[flip]) / static_cast<float>(a.D);
+    const float mean = row_sum<WARP>(dot, part_sum[flip]) * a.inv_d;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int e = first + i * step;
@@ -602,7 +616,7 @@ __global__ void __launch_bounds__(1024) rms_bwd_loop_kernel(const RowBwdArgs a) 
       dot = fmaf(t, w, dot);
     }
     first = false;
-    const float mean = row_sum<false>(dot, part_sum[flip]) / static_cast<float>(a.D);
+    const float mean = row_sum<false>(dot, part_sum[flip]) * a.inv_d;
     for (int c = threadIdx.x; c < D; c += blockDim.x) {
       float w;
       load_weight<DT, kSingle>(a.w, a.w_f32, c, D, &w);
@@ -613,20 +627,21 @@ __global__ void __launch_bounds__(1024) rms_bwd_loop_kernel(const RowBwdArgs a) 
   }
 }
 
-// dw[c] = sum over the CTAs' shares: 8 warps take every 8th share of 32 columns each, then the
-// eight sums are added in order.
-__global__ void __launch_bounds__(256) rms_dw_kernel(const float* part, int shares, int64_t D, void* dw, int dt) {
-  __shared__ float acc[8][32];
+// dw[c] = sum over the CTAs' shares: 32 warps take every 32nd share of 32 columns each, then the 32 sums
+// are added in order.
+constexpr int kDwWarps = 32;
+__global__ void __launch_bounds__(32 * kDwWarps) rms_dw_kernel(const float* part, int shares, int64_t D, void* dw, int dt) {
+  __shared__ float acc[kDwWarps][32];
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x;
   float sum = 0.f;
   if (c < D)
 #pragma unroll 8
-    for (int i = threadIdx.y; i < shares; i += 8) sum += part[static_cast<int64_t>(i) * D + c];
+    for (int i = threadIdx.y; i < shares; i += kDwWarps) sum += part[static_cast<int64_t>(i) * D + c];
   acc[threadIdx.y][threadIdx.x] = sum;
   __syncthreads();
   if (threadIdx.y == 0 && c < D) {
 #pragma unroll
-    for (int y = 1; y < 8; ++y) sum += acc[y][threadIdx.x];
+    for (int y = 1; y < kDwWarps; ++y) sum += acc[y][threadIdx.x];
     store_scalar_from_float(dw, c, dt, sum);
   }
 }
@@ -805,7 +820,7 @@ extern "C" int fmoe_rms_norm(const void* x, int64_t x_stride, const void* residu
   g.add(sum, D, T);
   g.add(y, D, T);
   g.weight(w);
-  const RowArgs a{x, residual, w, y, sum, rstd, q, q_scale, T, D, x_stride, r_stride, q_stride, eps, w_dtype == FMOE_F32,
+  const RowArgs a{x, residual, w, y, sum, rstd, q, q_scale, T, D, x_stride, r_stride, q_stride, eps, 1.0 / static_cast<double>(D), w_dtype == FMOE_F32,
                   g.shift0, g.shift_step};
   const RowShape s = row_shape(g, D, T, dtype);
   int rc = FMOE_OK;
@@ -825,7 +840,7 @@ extern "C" int fmoe_quantize_rows(const void* x, int64_t x_stride, int8_t* q, in
                "fmoe_quantize_rows: 8-bit rows must lie at 16-byte steps");
   RowGrid g(dtype);
   g.add(x, x_stride, T);
-  const RowArgs a{x, nullptr, nullptr, nullptr, nullptr, nullptr, q, q_scale, T, D, x_stride, 0, q_stride, 0.0, 0,
+  const RowArgs a{x, nullptr, nullptr, nullptr, nullptr, nullptr, q, q_scale, T, D, x_stride, 0, q_stride, 0.0, 0.0, 0,
                   g.shift0, g.shift_step};
   const RowShape s = row_shape(g, D, T, dtype);
   int rc = FMOE_OK;
@@ -883,11 +898,11 @@ extern "C" int fmoe_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* 
   if (bwd_smem(s, D, g.ve) > 220 * 1024) s.loop = true;  // fp32 rows of more than 14000 columns
   const int grid = s.loop ? bwd_grid_most(T, D) : bwd_grid(T, s.threads, s.warp);
   const RowBwdArgs a{dy, dsum, sum, rstd, w, dx, dw ? static_cast<float*>(scratch) : nullptr, T, D,
-                     dy_stride, ds_stride, s_stride, w_dtype == FMOE_F32, g.shift0, g.shift_step};
+                     dy_stride, ds_stride, s_stride, 1.f / static_cast<float>(D), w_dtype == FMOE_F32, g.shift0, g.shift_step};
   int rc = FMOE_OK;
   FMOE_DISPATCH_DTYPE(dtype, DT, rc = (launch_bwd<DT>(a, s, grid, st)));
   if (rc != 0 || dw == nullptr) return rc;
-  rms_dw_kernel<<<static_cast<unsigned>((D + 31) / 32), dim3(32, 8), 0, st>>>(static_cast<const float*>(scratch), grid, D, dw,
+  rms_dw_kernel<<<static_cast<unsigned>((D + 31) / 32), dim3(32, kDwWarps), 0, st>>>(static_cast<const float*>(scratch), grid, D, dw,
                                                                             w_dtype);
   return check_launch("rms_dw_kernel");
 }

@@ -42,11 +42,12 @@ def pack_activation(x: torch.Tensor) -> PackedActivation:
         raise ValueError(f"x must be float32/bfloat16/float16 rows, got {tuple(x.shape)} {x.dtype}")
     x2 = _rows(x.detach())
     T, D = x2.shape
-    q = torch.empty(T, _padded(D), dtype=torch.int8, device=x.device)
-    scale = torch.empty(T, (D + GROUP - 1) // GROUP, dtype=torch.float32, device=x.device)
-    ops._launch(x.device, "fmoe_pack_activation", 1, x2.data_ptr(), x2.stride(0), q.data_ptr(), q.stride(0),
+    Dp = _padded(D)
+    q = x2.new_empty((T, Dp), dtype=torch.int8)
+    scale = x2.new_empty((T, (D + GROUP - 1) // GROUP), dtype=torch.float32)
+    ops._launch(x.get_device(), "fmoe_pack_activation", 1, x2.data_ptr(), x2.stride(0), q.data_ptr(), Dp,
                 scale.data_ptr(), T, D, _DTYPES[x.dtype])  # fmt: skip
-    return PackedActivation(q[:, :D], scale, x.shape, x.dtype)
+    return PackedActivation(q if Dp == D else q[:, :D], scale, x.shape, x.dtype)
 
 
 def _check_packed(p: PackedActivation):
@@ -64,10 +65,10 @@ def _check_packed(p: PackedActivation):
 def unpack_activation(p: PackedActivation) -> torch.Tensor:
     """The values that `p` stands for, in the packed tensor's shape and type."""
     T, D = _check_packed(p)
-    out = torch.empty(T, D, dtype=p.dtype, device=p.q.device)
-    ops._launch(p.q.device, "fmoe_unpack_activation", 1, p.q.data_ptr(), p.q.stride(0), p.scale.data_ptr(),
+    out = p.q.new_empty((T, D), dtype=p.dtype)
+    ops._launch(p.q.get_device(), "fmoe_unpack_activation", 1, p.q.data_ptr(), p.q.stride(0), p.scale.data_ptr(),
                 out.data_ptr(), T, D, _DTYPES[p.dtype])  # fmt: skip
-    return out.view(p.shape)
+    return out if len(p.shape) == 2 else out.view(p.shape)
 
 
 def _backward(p, grad, act):
@@ -80,10 +81,12 @@ def _backward(p, grad, act):
         raise ValueError(f"grad must be {want} {p.dtype} on {p.q.device}, got {tuple(grad.shape)} {grad.dtype} "
                          f"on {grad.device}")  # fmt: skip
     g2 = _rows(grad.detach())
-    grad_h = torch.empty(T, D, dtype=p.dtype, device=p.q.device)
-    hidden = torch.empty(T, cols, dtype=p.dtype, device=p.q.device)
-    ops._launch(p.q.device, "fmoe_packed_act_bwd", 1, p.q.data_ptr(), p.q.stride(0), p.scale.data_ptr(), g2.data_ptr(),
+    grad_h = g2.new_empty((T, D))
+    hidden = g2.new_empty((T, cols))
+    ops._launch(p.q.get_device(), "fmoe_packed_act_bwd", 1, p.q.data_ptr(), p.q.stride(0), p.scale.data_ptr(), g2.data_ptr(),
                 g2.stride(0), grad_h.data_ptr(), hidden.data_ptr(), T, D, act, _DTYPES[p.dtype])  # fmt: skip
+    if len(want) == 2:
+        return grad_h, hidden
     return grad_h.view(p.shape), hidden.view(want)
 
 

@@ -56,6 +56,8 @@ class Int8Weight(NamedTuple):
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t as [T, D] rows with unit column stride, without a copy where its strides allow."""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
     if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
@@ -67,29 +69,28 @@ def _padded(K: int) -> int:
     return (K + 15) // 16 * 16
 
 
-def empty_rows(T: int, K: int, device) -> Int8Rows:
+def empty_rows(like: torch.Tensor, T: int, K: int) -> Int8Rows:
+    """Uninitialised 8-bit rows [T, K] and their scales, on the device of `like`."""
     Kp = _padded(K)
-    q = torch.empty(T, Kp, dtype=torch.int8, device=device)
-    return Int8Rows(q if Kp == K else q[:, :K], torch.empty(T, dtype=torch.float32, device=device))
-
-
-def _check_no_grad(t, what):
-    if torch.is_grad_enabled() and t.requires_grad:
-        raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+    q = like.new_empty((T, Kp), dtype=torch.int8)
+    return Int8Rows(q if Kp == K else q[:, :K], like.new_empty((T,), dtype=torch.float32))
 
 
 def quantize_rows(x: torch.Tensor) -> Int8Rows:
     """The rows (last dimension) of x in 8 bits: `q` [T, K] with T = all leading dimensions, `scale`
     float32 [T]."""
     _require_cuda(x, "x")
-    if x.dim() < 1 or x.dtype not in _DTYPES or x.shape[-1] == 0:
+    dtype = _DTYPES.get(x.dtype)
+    if dtype is None or x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"x must be float32/bfloat16/float16 rows, got {tuple(x.shape)} {x.dtype}")
-    _check_no_grad(x, "quantize_rows")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("quantize_rows has no gradient: call it under torch.no_grad() or on detached tensors")
     x2 = _rows(x)
     T, K = x2.shape
-    out = empty_rows(T, K, x.device)
-    ops._launch(x.device, "fmoe_quantize_rows", 1, x2.data_ptr(), x2.stride(0), out.q.data_ptr(), out.q.stride(0),
-                out.scale.data_ptr(), T, K, _DTYPES[x2.dtype])  # fmt: skip
+    out = empty_rows(x2, T, K)
+    q, scale = out
+    ops._launch(x.get_device(), "fmoe_quantize_rows", 1, x2.data_ptr(), x2.stride(0), q.data_ptr(), q.stride(0),
+                scale.data_ptr(), T, K, dtype)  # fmt: skip
     return out
 
 
@@ -101,9 +102,9 @@ def dequantize_rows(rows: Int8Rows, dtype: torch.dtype = torch.bfloat16) -> torc
         raise ValueError(f"unsupported dtype {dtype}; use float32, bfloat16 or float16")
     q, scale = _rows(q), scale.contiguous()
     T, K = q.shape
-    out = torch.empty(T, K, dtype=dtype, device=q.device)
-    ops._launch(q.device, "fmoe_dequantize_rows", 1, q.data_ptr(), q.stride(0), scale.data_ptr(),
-                out.data_ptr(), T, K, _DTYPES[dtype])  # fmt: skip
+    out = q.new_empty((T, K), dtype=dtype)
+    ops._launch(q.get_device(), "fmoe_dequantize_rows", 1, q.data_ptr(), q.stride(0), scale.data_ptr(), out.data_ptr(), T, K,
+                _DTYPES[dtype])  # fmt: skip
     return out
 
 
@@ -121,23 +122,24 @@ def _check_rows(q, scale):
     _require_cuda(q, "q")
     if q.dtype != torch.int8 or q.dim() != 2 or q.shape[1] == 0:
         raise ValueError(f"q must be int8 [T, K], got {tuple(q.shape)} {q.dtype}")
-    if scale.dtype != torch.float32 or scale.shape != q.shape[:-1] or scale.device != q.device:
-        raise ValueError(f"scale must be float32 {tuple(q.shape[:-1])} on {q.device}, got {tuple(scale.shape)} "
+    if scale.dtype != torch.float32 or scale.shape != q.shape[:1] or scale.get_device() != q.get_device():
+        raise ValueError(f"scale must be float32 {tuple(q.shape[:1])} on {q.device}, got {tuple(scale.shape)} "
                          f"{scale.dtype} on {scale.device}")  # fmt: skip
 
 
 def _operand(q: torch.Tensor) -> torch.Tensor:
     """q with rows at 16-byte steps and readable up to the last step: q itself where its strides and
     storage say so (what the functions above return), else a padded copy."""
-    K = q.shape[-1]
-    lead = q.shape[:-1]
-    rows = q.shape[-2]
-    ok = (K == 1 or q.stride(-1) == 1) and q.data_ptr() % 16 == 0
-    ok = ok and q.stride(-2) % 16 == 0 and q.stride(-2) >= K
-    if q.dim() == 3:
-        ok = ok and q.stride(0) % 16 == 0 and q.stride(0) >= rows * q.stride(-2)
+    shape = q.shape
+    K = shape[-1]
+    if K % 16 == 0 and q.is_contiguous() and q.data_ptr() % 16 == 0:
+        return q
+    lead, strides = shape[:-1], q.stride()
+    ok = (K == 1 or strides[-1] == 1) and q.data_ptr() % 16 == 0 and strides[-2] % 16 == 0 and strides[-2] >= K
+    if len(shape) == 3:
+        ok = ok and strides[0] % 16 == 0 and strides[0] >= shape[-2] * strides[-2]
     if ok and K % 16:
-        last = q.storage_offset() + sum((n - 1) * s for n, s in zip(lead, q.stride()[:-1])) + _padded(K)
+        last = q.storage_offset() + sum((n - 1) * s for n, s in zip(lead, strides[:-1])) + _padded(K)
         ok = last <= q.untyped_storage().nbytes()
     if ok or q.numel() == 0:
         return q
@@ -149,33 +151,37 @@ def _operand(q: torch.Tensor) -> torch.Tensor:
 def _product(a, w, offsets, counts, act, out, E):
     # held in names until the launch: a copy made only for its address would be freed before it
     aq, wq, sa, sw = _operand(a.q), _operand(w.q), a.scale.contiguous(), w.scale.contiguous()
-    N, K = wq.shape[-2:]
-    dev = aq.device
+    wshape, wstride = wq.shape, wq.stride()
+    N, K = wshape[-2:]
+    R = aq.shape[0]
+    dev = aq.get_device()
     ops._launch(
-        dev, "fmoe_int8_gemm", 1, aq.data_ptr(), aq.stride(0) if aq.shape[0] > 1 else _padded(K),
-        sa.data_ptr(), wq.data_ptr(), wq.stride(-2), wq.stride(0) if wq.dim() == 3 else 0,
-        sw.data_ptr(), out.data_ptr(), None if offsets is None else offsets.data_ptr(),
-        None if counts is None else counts.data_ptr(), E, aq.shape[0], N, K, act, _DTYPES[out.dtype],
-        _status_word(dev).data_ptr(),
+        dev, "fmoe_int8_gemm", 1, aq.data_ptr(), aq.stride(0) if R > 1 else _padded(K), sa.data_ptr(), wq.data_ptr(),
+        wstride[-2], wstride[0] if len(wshape) == 3 else 0, sw.data_ptr(), out.data_ptr(),
+        None if offsets is None else offsets.data_ptr(), None if counts is None else counts.data_ptr(), E, R, N, K, act,
+        _DTYPES[out.dtype], _status_word(aq.device).data_ptr(),
     )  # fmt: skip
-    ops._maybe_check(dev, "fmoe_int8_gemm")
+    ops._maybe_check(aq.device, "fmoe_int8_gemm")
     return out
 
 
 def _check_operands(a, w, dims, out_dtype):
-    _check_rows(a.q, a.scale)
-    _require_cuda(w.q, "w")
-    if w.q.dtype != torch.int8 or w.q.dim() != dims or w.q.shape[-1] != a.q.shape[1]:
+    q, wq, ws = a.q, w.q, w.scale
+    _check_rows(q, a.scale)
+    _require_cuda(wq, "w")
+    wshape, K = wq.shape, q.shape[1]
+    if wq.dtype != torch.int8 or len(wshape) != dims or wshape[-1] != K:
         raise ValueError(f"a must be int8 [R, K] and w int8 {'[E, N, K]' if dims == 3 else '[N, K]'}; got "
-                         f"{tuple(a.q.shape)} and {tuple(w.q.shape)} {w.q.dtype}")  # fmt: skip
-    if w.scale.dtype != torch.float32 or w.scale.shape != w.q.shape[:-1]:
-        raise ValueError(f"w's scale must be float32 {tuple(w.q.shape[:-1])}, got {tuple(w.scale.shape)} {w.scale.dtype}")
-    if w.q.device != a.q.device or w.scale.device != a.q.device:
-        raise ValueError(f"a lives on {a.q.device}, w on {w.q.device} and {w.scale.device}")
-    if w.q.shape[-2] == 0:
+                         f"{tuple(q.shape)} and {tuple(wshape)} {wq.dtype}")  # fmt: skip
+    if ws.dtype != torch.float32 or ws.shape != wshape[:-1]:
+        raise ValueError(f"w's scale must be float32 {tuple(wshape[:-1])}, got {tuple(ws.shape)} {ws.dtype}")
+    dev = q.get_device()
+    if wq.get_device() != dev or ws.get_device() != dev:
+        raise ValueError(f"a lives on {q.device}, w on {wq.device} and {ws.device}")
+    if wshape[-2] == 0:
         raise ValueError("w has no output channels")
-    if a.q.shape[1] > MAX_K:
-        raise ValueError(f"K={a.q.shape[1]} could overflow the 32-bit sums (K <= {MAX_K})")
+    if K > MAX_K:
+        raise ValueError(f"K={K} could overflow the 32-bit sums (K <= {MAX_K})")
     if out_dtype not in _DTYPES:
         raise ValueError(f"unsupported out_dtype {out_dtype}; use float32, bfloat16 or float16")
 
@@ -183,7 +189,7 @@ def _check_operands(a, w, dims, out_dtype):
 def int8_linear(a: Int8Rows, w: Int8Weight, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """a [T, K] times w [N, K] transposed, both in 8 bits: [T, N] in `out_dtype`, rounded once."""
     _check_operands(a, w, 2, out_dtype)
-    out = torch.empty(a.q.shape[0], w.q.shape[0], dtype=out_dtype, device=a.q.device)
+    out = a.q.new_empty((a.q.shape[0], w.q.shape[0]), dtype=out_dtype)
     return _product(a, w, None, None, _lib.ACT_NONE, out, 1)
 
 
@@ -207,8 +213,8 @@ def grouped_int8_gemm(a: Int8Rows, w: Int8Weight, offsets, counts, activation: i
         if t.dtype != torch.int64 or t.shape != (E,) or t.device != a.q.device:
             raise ValueError(f"{name} must be int64 [{E}] on {a.q.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
     cols = N // 2 if act == _lib.ACT_SWIGLU else N
-    alloc = torch.empty if covers_all_rows else torch.zeros
-    out = alloc(a.q.shape[0], cols, dtype=out_dtype, device=a.q.device)
+    alloc = a.q.new_empty if covers_all_rows else a.q.new_zeros
+    out = alloc((a.q.shape[0], cols), dtype=out_dtype)
     if E == 0:
         return out
     return _product(a, w, offsets.contiguous(), counts.contiguous(), act, out, E)

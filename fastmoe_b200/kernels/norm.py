@@ -36,21 +36,23 @@ class NormInt8(NamedTuple):
 def _check(x, weight, residual, eps):
     _require_cuda(x, "x")
     _require_cuda(weight, "weight")
-    if x.dim() < 1 or x.dtype not in _DTYPES:
-        raise ValueError(f"x must be float32/bfloat16/float16 rows, got {tuple(x.shape)} {x.dtype}")
-    D = x.shape[-1]
+    dtype, shape = x.dtype, x.shape
+    if len(shape) < 1 or dtype not in _DTYPES:
+        raise ValueError(f"x must be float32/bfloat16/float16 rows, got {tuple(shape)} {dtype}")
+    D = shape[-1]
     if D == 0:
         raise ValueError("rows of width 0 have no norm")
-    if weight.shape != (D,) or weight.dtype not in (x.dtype, torch.float32) or weight.device != x.device:
+    dev = x.get_device()
+    if weight.shape != (D,) or weight.dtype not in (dtype, torch.float32) or weight.get_device() != dev:
         raise ValueError(
-            f"weight must be a [{D}] vector of {x.dtype} or float32 on {x.device}, got {tuple(weight.shape)} "
+            f"weight must be a [{D}] vector of {dtype} or float32 on {x.device}, got {tuple(weight.shape)} "
             f"{weight.dtype} on {weight.device}"
         )
     if residual is not None and (
-        residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device
+        residual.shape != shape or residual.dtype != dtype or residual.get_device() != dev
     ):
         raise ValueError(
-            f"residual must match x ({tuple(x.shape)}, {x.dtype}, {x.device}), got {tuple(residual.shape)}, "
+            f"residual must match x ({tuple(shape)}, {dtype}, {x.device}), got {tuple(residual.shape)}, "
             f"{residual.dtype}, {residual.device}"
         )
     if not eps >= 0.0:
@@ -59,20 +61,54 @@ def _check(x, weight, residual, eps):
 
 def _forward(x2, r2, weight, eps, want_y, want_rstd, want_q):
     """One launch over [T, D] rows; returns (y, stream, rstd, Int8Rows)."""
-    T, D = x2.shape
-    dev = x2.device
-    y = torch.empty(T, D, dtype=x2.dtype, device=dev) if want_y else None
-    stream = torch.empty(T, D, dtype=x2.dtype, device=dev) if r2 is not None else None
-    rstd = torch.empty(T, dtype=torch.float32, device=dev) if want_rstd else None
-    q = empty_rows(T, D, dev) if want_q else None
+    T, D = shape = x2.shape
+    dtype = _DTYPES[x2.dtype]
+    y = x2.new_empty(shape) if want_y else None
+    stream = x2.new_empty(shape) if r2 is not None else None
+    rstd = x2.new_empty((T,), dtype=torch.float32) if want_rstd else None
+    rows = empty_rows(x2, T, D) if want_q else None
     ops._launch(
-        dev, "fmoe_rms_norm", 1, x2.data_ptr(), x2.stride(0), None if r2 is None else r2.data_ptr(),
+        x2.get_device(), "fmoe_rms_norm", 1, x2.data_ptr(), x2.stride(0), None if r2 is None else r2.data_ptr(),
         0 if r2 is None else r2.stride(0), weight.data_ptr(), _DTYPES[weight.dtype],
         None if y is None else y.data_ptr(), None if stream is None else stream.data_ptr(),
-        None if rstd is None else rstd.data_ptr(), None if q is None else q.q.data_ptr(),
-        0 if q is None else q.q.stride(0), None if q is None else q.scale.data_ptr(), T, D, eps, _DTYPES[x2.dtype],
+        None if rstd is None else rstd.data_ptr(), None if rows is None else rows.q.data_ptr(),
+        0 if rows is None else rows.q.stride(0), None if rows is None else rows.scale.data_ptr(), T, D, eps, dtype,
     )  # fmt: skip
-    return y, stream, rstd, q
+    return y, stream, rstd, rows
+
+
+def _shaped(t, shape):
+    return t if t.shape == shape else t.view(shape)
+
+
+def _rms_backward(ctx, dy, dstream=None):
+    if dy is None:  # the normed rows were not used: the stream's gradient passes through
+        return dstream, dstream if ctx.needs_input_grad[1] else None, None, None
+    s, rstd, weight = ctx.saved_tensors
+    T, D = s.shape
+    dy2 = _rows(dy if dy.dtype == s.dtype else dy.to(s.dtype))
+    ds2 = None
+    if dstream is not None:
+        ds2 = _rows(dstream if dstream.dtype == s.dtype else dstream.to(s.dtype))
+    dx = s.new_empty((T, D))
+    dw = scratch = None
+    nbytes = 0
+    if ctx.needs_input_grad[2]:
+        dw = weight.new_empty(weight.shape)
+        nbytes = _lib.lib().fmoe_rms_norm_bwd_bytes(T, D)
+        scratch = s.new_empty((nbytes,), dtype=torch.uint8)
+    ops._launch(
+        s.get_device(), "fmoe_rms_norm_bwd", 1 if dw is None else 2, dy2.data_ptr(), dy2.stride(0),
+        None if ds2 is None else ds2.data_ptr(), 0 if ds2 is None else ds2.stride(0), s.data_ptr(), s.stride(0),
+        rstd.data_ptr(), weight.data_ptr(), _DTYPES[weight.dtype], dx.data_ptr(),
+        None if dw is None else dw.data_ptr(), None if scratch is None else scratch.data_ptr(), nbytes, T, D,
+        _DTYPES[s.dtype],
+    )  # fmt: skip
+    dx = _shaped(dx, ctx.shape)
+    return dx, dx if ctx.needs_input_grad[1] else None, dw, None
+
+
+_rms_backward_once = once_differentiable(_rms_backward)
 
 
 class _RmsNorm(torch.autograd.Function):
@@ -83,36 +119,15 @@ class _RmsNorm(torch.autograd.Function):
         x2 = _rows(x)
         y, stream, rstd, _ = _forward(x2, None if residual is None else _rows(residual), weight, eps, True, True, False)
         ctx.save_for_backward(x2 if stream is None else stream, rstd, weight)
-        ctx.shape = x.shape
+        ctx.shape = shape = x.shape
         if stream is None:
-            return y.view(x.shape)
-        return y.view(x.shape), stream.view(x.shape)
+            return _shaped(y, shape)
+        return _shaped(y, shape), _shaped(stream, shape)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dstream=None):
-        s, rstd, weight = ctx.saved_tensors
-        if dy is None:  # the normed rows were not used: the stream's gradient passes through
-            return dstream, dstream if ctx.needs_input_grad[1] else None, None, None
-        T, D = s.shape
-        dy2 = _rows(dy.to(s.dtype))
-        ds2 = None if dstream is None else _rows(dstream.to(s.dtype))
-        dx = torch.empty(T, D, dtype=s.dtype, device=s.device)
-        dw = scratch = None
-        nbytes = 0
-        if ctx.needs_input_grad[2]:
-            dw = torch.empty_like(weight)
-            nbytes = _lib.lib().fmoe_rms_norm_bwd_bytes(T, D)
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=s.device)
-        ops._launch(
-            s.device, "fmoe_rms_norm_bwd", 1 if dw is None else 2, dy2.data_ptr(), dy2.stride(0),
-            None if ds2 is None else ds2.data_ptr(), 0 if ds2 is None else ds2.stride(0), s.data_ptr(), s.stride(0),
-            rstd.data_ptr(), weight.data_ptr(), _DTYPES[weight.dtype], dx.data_ptr(),
-            None if dw is None else dw.data_ptr(), None if scratch is None else scratch.data_ptr(), nbytes, T, D,
-            _DTYPES[s.dtype],
-        )  # fmt: skip
-        dx = dx.view(ctx.shape)
-        return dx, dx if ctx.needs_input_grad[1] else None, dw, None
+    def backward(ctx, *grads):
+        # there is no second derivative: under create_graph the result is marked so
+        return (_rms_backward_once if torch.is_grad_enabled() else _rms_backward)(ctx, *grads)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
