@@ -24,10 +24,9 @@ extern int g_gemm_sms, g_gemm_skip_loads, g_gemm_spin_limit;
 
 namespace i8 {
 
-constexpr int kBM = 128, kBN = 256, kBK = 128, kStages = 4, kUmmaK = 32;
+constexpr int kBM = 128, kBN = 256, kBK = 128, kUmmaK = 32;
 constexpr int kABytes = kBM * kBK;  // 16 KB
-constexpr int kBBytes = kBN * kBK;  // 32 KB
-constexpr int kStageBytes = kABytes + kBBytes;
+constexpr int kPipeBytes = 4 * 48 * 1024;  // pipeline of int8_gemm_kernel: 4 stages, or 6 of a pair
 constexpr int kThreads = 192;      // int8_tn_kernel
 constexpr int kEpiWarps = 8;       // of int8_gemm_kernel: two per quarter of tensor memory, half of the columns each
 constexpr int kTileThreads = 64 + 32 * kEpiWarps;
@@ -53,8 +52,73 @@ struct Args {
   int32_t* status;
 };
 
-// Instruction descriptor: D s32, A and B signed 8 bits, both K-major, M=128, N=256.
+// Instruction descriptor: D s32, A and B signed 8 bits, both K-major, M=128 (256 for a pair), N=256.
 constexpr uint32_t kIdesc = (2u << 4) | (1u << 7) | (1u << 10) | ((kBN >> 3) << 17) | ((kBM >> 4) << 24);
+constexpr uint32_t kIdescPair = (2u << 4) | (1u << 7) | (1u << 10) | ((kBN >> 3) << 17) | ((2 * kBM >> 4) << 24);
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address, in the cluster's window, of CTA 0's copy of a shared-memory object.
+__device__ __forceinline__ uint32_t leader_addr(const void* p) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_leader(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
+}
+// mbar_wait for arrivals from the other CTA of the cluster.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t limit) {
+  const uint32_t addr = smem_u32(bar);
+  for (uint32_t spin = 0; spin < limit; ++spin) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((spin & 1023u) == 1023u && *abort_flag) return false;
+  }
+  return false;
+}
+// Loads of a pair: into this CTA's memory, counted by the leader's barrier.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(kIdescPair), "r"(accumulate)
+      : "memory");
+}
+// Arrives on `bar` of both CTAs once every MMA issued so far has completed.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
 
 __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
                                         uint32_t accumulate) {
@@ -85,6 +149,7 @@ struct Tile {
 // about kRowGroup row blocks and 148 / kRowGroup column blocks: 36 MB of operands at K = 8192,
 // which L2 holds, where one column block against all rows of a 32768-row matrix would stream
 // 268 MB of rows per column block.
+template <int BM>
 __device__ __forceinline__ Tile locate(int tile, const int* mb_prefix, const Args& a) {
   int lo = 0, hi = a.E;
   while (hi - lo > 1) {
@@ -93,39 +158,51 @@ __device__ __forceinline__ Tile locate(int tile, const int* mb_prefix, const Arg
   }
   const int mblocks = mb_prefix[lo + 1] - mb_prefix[lo];
   int local = tile - mb_prefix[lo] * a.n_blocks;
-  const int group = local / (kRowGroup * a.n_blocks);
-  local -= group * kRowGroup * a.n_blocks;
-  const int left = mblocks - group * kRowGroup;
-  const int height = left < kRowGroup ? left : kRowGroup;
+  constexpr int kHeight = kRowGroup * kBM / BM;
+  const int group = local / (kHeight * a.n_blocks);
+  local -= group * kHeight * a.n_blocks;
+  const int left = mblocks - group * kHeight;
+  const int height = left < kHeight ? left : kHeight;
   Tile t;
   t.expert = lo;
   t.nb = local / height;
-  const int64_t first = static_cast<int64_t>(group * kRowGroup + local - t.nb * height) * kBM;
+  const int64_t first = static_cast<int64_t>(group * kHeight + local - t.nb * height) * BM;
   t.row0 = (a.offsets == nullptr ? 0 : a.offsets[lo]) + first;
   const int64_t rows = rows_of(a, lo) - first;
-  t.rows = static_cast<int>(rows < kBM ? rows : kBM);
+  t.rows = static_cast<int>(rows < BM ? rows : BM);
   return t;
 }
 
-template <int DT>
+// PAIR: two CTAs of a cluster share a tile of 256 rows. Each loads its own 128 rows and half of the 256
+// weight rows (32 KB per 128 bytes of K instead of 48: at 64 bytes a clock and SM the tensor pipe
+// otherwise waits for its operands), CTA 0 issues the MMAs of both, and each keeps its rows'
+// accumulators and writes them out. Barriers: `full` of CTA 0 counts the bytes of both; `empty` and
+// `tmem_full` of each are arrived on by CTA 0's commits; `tmem_empty` of CTA 0 by the epilogue warps
+// of both.
+template <int DT, bool PAIR>
 __global__ void __launch_bounds__(kTileThreads, 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                      const Args a) {
+  constexpr int kRows = PAIR ? 2 * kBM : kBM;              // rows of a tile
+  constexpr int kBBytes = (PAIR ? kBN / 2 : kBN) * kBK;    // weights this CTA loads per stage
+  constexpr int kStageBytes = kABytes + kBBytes, kStages = kPipeBytes / kStageBytes;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* smem_a = smem;
   uint8_t* smem_b = smem + kStages * kABytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPipeBytes);
   uint64_t* empty = full + kStages;
   uint64_t* tmem_full = empty + kStages;
   uint64_t* tmem_empty = tmem_full + 2;
   uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
   int* abort_flag = reinterpret_cast<int*>(tmem_base_slot + 1);
   uint64_t* drain = reinterpret_cast<uint64_t*>(abort_flag + 1);
-  uint4* stage_buf = reinterpret_cast<uint4*>(smem + kStages * kStageBytes + 256);
-  int* mb_prefix = reinterpret_cast<int*>(smem + kStages * kStageBytes + 256 + kEpiStageBytes);  // [E + 1]
+  uint4* stage_buf = reinterpret_cast<uint4*>(smem + kPipeBytes + 256);
+  int* mb_prefix = reinterpret_cast<int*>(smem + kPipeBytes + 256 + kEpiStageBytes);  // [E + 1]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = PAIR ? static_cast<int>(cluster_rank()) : 0;
+  const int worker = static_cast<int>(blockIdx.x) / (PAIR ? 2 : 1), workers = static_cast<int>(gridDim.x) / (PAIR ? 2 : 1);
   const bool swiglu = a.act == FMOE_ACT_SWIGLU;
   int fills = 0;
   bool mma_issued = false;
@@ -135,7 +212,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int64_t n = rows_of(a, e);
     if (a.counts != nullptr && n != a.counts[e] && a.counts[e] > 0 && a.status != nullptr && blockIdx.x == 0)
       atomicOr(a.status, FMOE_STATUS_BAD_EXPERT);  // rows past the end of A were cut off
-    mb_prefix[e + 1] = static_cast<int>((n + kBM - 1) / kBM);
+    mb_prefix[e + 1] = static_cast<int>((n + kRows - 1) / kRows);
   }
   if (threadIdx.x == 0) {
     mb_prefix[0] = 0;
@@ -146,7 +223,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tmem_full[i], 1);
-      mbar_init(&tmem_empty[i], kEpiWarps);
+      mbar_init(&tmem_empty[i], (PAIR ? 2 : 1) * kEpiWarps);
     }
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -167,12 +244,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_base_slot))
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_base_slot))
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_base_slot))
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   tcgen05_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();  // both CTAs' barriers are set up before either is signalled
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_base_slot;
   const int total_tiles = mb_prefix[a.E] * a.n_blocks;
@@ -181,46 +265,60 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     // ---- TMA producer ---------------------------------------------------------------
     int stage = 0;
     uint32_t phase = 0;
-    for (int tile = blockIdx.x; tile < total_tiles && !a.skip_loads; tile += gridDim.x) {
-      const Tile t = locate(tile, mb_prefix, a);
+    for (int tile = worker; tile < total_tiles && !a.skip_loads; tile += workers) {
+      const Tile t = locate<kRows>(tile, mb_prefix, a);
       for (int kb = 0; kb < a.k_blocks; ++kb) {
-        if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, a.spin_limit)) goto timed_out;
-        mbar_expect_tx(&full[stage], kStageBytes);
-        tma_load_2d(smem_a + stage * kABytes, &map_a, kb * kBK, static_cast<int>(t.row0), &full[stage]);
-        uint8_t* b = smem_b + stage * kBBytes;
-        if (swiglu) {  // 128 gate rows, then the up rows of the same columns
-          tma_load_3d(b, &map_w, kb * kBK, t.nb * 128, t.expert, &full[stage]);
-          tma_load_3d(b + kBBytes / 2, &map_w, kb * kBK, static_cast<int>(a.cols) + t.nb * 128, t.expert, &full[stage]);
+        if constexpr (PAIR) {
+          if (!mbar_wait_cluster(&empty[stage], phase ^ 1, abort_flag, a.spin_limit)) goto timed_out;
+          if (rank == 0) mbar_expect_tx(&full[stage], 2 * kStageBytes);
+          const uint32_t bar = leader_addr(&full[stage]);
+          tma_load_2d_pair(smem_a + stage * kABytes, &map_a, kb * kBK, static_cast<int>(t.row0) + rank * kBM, bar);
+          // columns 0 .. 127 of the tile are CTA 0's, 128 .. 255 (the up rows for SwiGLU) CTA 1's
+          const int w_row = swiglu ? rank * static_cast<int>(a.cols) + t.nb * 128 : t.nb * kBN + rank * 128;
+          tma_load_3d_pair(smem_b + stage * kBBytes, &map_w, kb * kBK, w_row, t.expert, bar);
         } else {
-          tma_load_3d(b, &map_w, kb * kBK, t.nb * kBN, t.expert, &full[stage]);
+          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, a.spin_limit)) goto timed_out;
+          mbar_expect_tx(&full[stage], kStageBytes);
+          tma_load_2d(smem_a + stage * kABytes, &map_a, kb * kBK, static_cast<int>(t.row0), &full[stage]);
+          uint8_t* b = smem_b + stage * kBBytes;
+          if (swiglu) {  // 128 gate rows, then the up rows of the same columns
+            tma_load_3d(b, &map_w, kb * kBK, t.nb * 128, t.expert, &full[stage]);
+            tma_load_3d(b + kBBytes / 2, &map_w, kb * kBK, static_cast<int>(a.cols) + t.nb * 128, t.expert, &full[stage]);
+          } else {
+            tma_load_3d(b, &map_w, kb * kBK, t.nb * kBN, t.expert, &full[stage]);
+          }
         }
         ++fills;
         if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
     }
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1 && lane == 0 && rank == 0) {
     // ---- MMA issuer -----------------------------------------------------------------
     int stage = 0;
     uint32_t phase = 0;
     int it = 0;
-    for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++it) {
+    for (int tile = worker; tile < total_tiles; tile += workers, ++it) {
       const int acc = it & 1;
-      if (!mbar_wait(&tmem_empty[acc], ((it >> 1) & 1) ^ 1, abort_flag, a.spin_limit)) goto timed_out;
+      if (!mbar_wait_cluster(&tmem_empty[acc], ((it >> 1) & 1) ^ 1, abort_flag, a.spin_limit)) goto timed_out;
       tcgen05_fence_after();
       const uint32_t tmem_d = tmem_base + acc * kBN;
       for (int kb = 0; kb < a.k_blocks; ++kb) {
-        if (!mbar_wait(&full[stage], phase, abort_flag, a.spin_limit)) goto timed_out;
+        if (!mbar_wait_cluster(&full[stage], phase, abort_flag, a.spin_limit)) goto timed_out;
         tcgen05_fence_after();
         mma_issued = true;
         const uint64_t da = smem_desc(smem_u32(smem_a + stage * kABytes));
         const uint64_t db = smem_desc(smem_u32(smem_b + stage * kBBytes));
 #pragma unroll
-        for (int k = 0; k < kBK / kUmmaK; ++k)  // 32 bytes along K inside the swizzle atom: +2 encoded
-          umma_i8(tmem_d, da + 2 * k, db + 2 * k, kIdesc, (kb | k) != 0 ? 1u : 0u);
-        umma_commit(&empty[stage]);
+        for (int k = 0; k < kBK / kUmmaK; ++k) {  // 32 bytes along K inside the swizzle atom: +2 encoded
+          if constexpr (PAIR) umma_i8_pair(tmem_d, da + 2 * k, db + 2 * k, (kb | k) != 0 ? 1u : 0u);
+          else umma_i8(tmem_d, da + 2 * k, db + 2 * k, kIdesc, (kb | k) != 0 ? 1u : 0u);
+        }
+        if constexpr (PAIR) umma_commit_pair(&empty[stage]);
+        else umma_commit(&empty[stage]);
         if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
-      umma_commit(&tmem_full[acc]);
+      if constexpr (PAIR) umma_commit_pair(&tmem_full[acc]);
+      else umma_commit(&tmem_full[acc]);
     }
   } else if (warp >= 2) {
     // ---- epilogue -------------------------------------------------------------------
@@ -231,14 +329,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     uint4* stage_w = stage_buf + (warp - 2) * (32 * 4);
     const int out_cols = swiglu ? 128 : kBN;
     int it = 0;
-    for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++it) {
+    for (int tile = worker; tile < total_tiles; tile += workers, ++it) {
       const int acc = it & 1;
-      const Tile t = locate(tile, mb_prefix, a);
+      Tile t = locate<kRows>(tile, mb_prefix, a);
+      t.row0 += rank * kBM;  // this CTA's half of a pair's rows
+      t.rows -= rank * kBM;
       const int row = quarter * 32 + lane;
       const int warp_rows = t.rows - quarter * 32;  // valid rows of this warp (may be <= 0)
       const float sa = row < t.rows ? a.a_scale[t.row0 + row] : 0.f;
       const float* sw = a.w_scale + static_cast<int64_t>(t.expert) * a.N;
-      if (!mbar_wait(&tmem_full[acc], (it >> 1) & 1, abort_flag, a.spin_limit)) goto timed_out;
+      if (!mbar_wait_cluster(&tmem_full[acc], (it >> 1) & 1, abort_flag, a.spin_limit)) goto timed_out;
       tcgen05_fence_after();
       const uint32_t taddr = tmem_base + acc * kBN + (static_cast<uint32_t>(quarter * 32) << 16);
       const int c_end = (half + 1) * (out_cols / 2);
@@ -304,7 +404,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tmem_empty[acc]);
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_leader(&tmem_empty[acc]);
+        else mbar_arrive(&tmem_empty[acc]);
+      }
     }
   }
   goto done;
@@ -314,13 +417,36 @@ timed_out:
   if (a.status != nullptr) atomicOr(a.status, FMOE_STATUS_WAIT_TIMEOUT);
 
 done:
-  drain_on_exit(warp, lane, fills, mma_issued, full, drain, abort_flag, kStages, a.spin_limit);
+  if constexpr (PAIR) {
+    // CTA 0 sees the pair's loads land and its MMAs finish; CTA 1 waits for it at the cluster's barrier,
+    // after which nothing is on its way into either CTA's memory.
+    if (rank == 0 && warp == 0 && lane == 0 && *abort_flag) {
+      for (int s = 0; s < kStages && s < fills; ++s) {
+        const int last = (fills - 1 - s) / kStages * kStages + s;  // last fill that used stage s
+        mbar_wait_plain(&full[s], (last / kStages) & 1, a.spin_limit);
+      }
+    }
+    if (mma_issued) {
+      umma_commit_pair(drain);
+      mbar_wait_plain(drain, 0, a.spin_limit);
+    }
+  } else {
+    drain_on_exit(warp, lane, fills, mma_issued, full, drain, abort_flag, kStages, a.spin_limit);
+  }
   tcgen05_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();
   if (warp == 1) {
     __syncwarp();
     tcgen05_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
+    if constexpr (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
+  }
+  if constexpr (PAIR) {
+    __syncwarp();
+    cluster_sync_all();  // neither leaves before both have given the tensor memory back
   }
 }
 
@@ -541,15 +667,6 @@ struct TnArgs {
   int splits;    // CTAs per cluster, each with its share of K; 1: a persistent grid
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // Four integers at `saddr` of CTA `rank`'s shared memory. Not volatile: the loads of one output go out
 // together. (A volatile load per CTA and output, one after the other, cost 20 us at 128 tokens.)
 __device__ __forceinline__ int4 ld_cluster4(uint32_t saddr, uint32_t rank) {
@@ -903,6 +1020,29 @@ static int launch_tn(const CUtensorMap& map_t, const CUtensorMap& map_w, const T
   return check_launch("int8_tn_kernel");
 }
 
+template <int DT, bool PAIR>
+static int launch_tiles(const CUtensorMap& map_a, const CUtensorMap& map_w, const Args& g, cudaStream_t st) {
+  constexpr int kFixed = 1024 + kPipeBytes + 256 + kEpiStageBytes, kRows = PAIR ? 2 * kBM : kBM, kCtas = PAIR ? 2 : 1;
+  FMOE_CUDA(cudaFuncSetAttribute(int8_gemm_kernel<DT, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kFixed + static_cast<int>(sizeof(int)) * (kMaxExperts + 2)));
+  // upper bound of the tile count, known without reading the counts: one partial block per expert
+  const int64_t tiles = ((g.R + kRows - 1) / kRows + g.E - 1) * g.n_blocks;
+  const int64_t most = g_gemm_sms / kCtas > 0 ? g_gemm_sms / kCtas : 1;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(static_cast<unsigned>(kCtas * (tiles < most ? tiles : most)));
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = kFixed + sizeof(int) * (g.E + 2);
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCtas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 1 : 0;
+  FMOE_CUDA(cudaLaunchKernelEx(&cfg, int8_gemm_kernel<DT, PAIR>, map_a, map_w, g));
+  return check_launch("int8_gemm_kernel");
+}
+
 }  // namespace i8
 
 int g_int8_few_rows = -1;  // fmoe_tune "int8_few_rows": 1 / 0 forces the kernel, -1 = by the sizes
@@ -964,8 +1104,11 @@ extern "C" int fmoe_int8_gemm(const int8_t* a, int64_t a_stride, const float* a_
     // (few / split K / tiled, us): 512 x 4096, 8 rows 3.4 / 5.8 / 8.8, 64 rows 7.9 / 9.1 / 9.2; 2048 x 7168, 8
     // rows 6.6 / 8.9 / 16.6, 24 rows 11.3 / 9.5 / 17.0. A tile of the tiled kernel takes the same time for 1 row
     // and for 128, so it needs tiles for most SMs: 7168 x 7168, 256 rows (56 tiles) - / 26 / 33, 512 rows
-    // (112) - / 35 / 32; 64 experts of 7168 x 4096, 32 rows each - / 282 / 292, 128 each - / 359 / 339.
-    which = tokens <= i8::kFewTokens && (tokens + 7) / 8 * touched <= i8::kFewBytes ? 1 : mean <= 64 || tiles <= 56 ? 2 : 0;
+    // (112) - / 35 / 32; 64 experts of 7168 x 4096, 32 rows each - / 282 / 292, 128 each - / 359 / 339. Pairs of CTAs: 8192 x 8192,
+    // 1024 rows 57 -> 52, 32768 rows for seconds on end (at the power limit) 1680 -> 1620; their 256-row tiles pad
+    // an expert of a few hundred rows more than that gains (32 experts of 7168 x 4096, 256 rows 263 -> 292, 1024
+    // rows 726 -> 725, 2048 rows for seconds on end 1490 -> 1440).
+    which = tokens <= i8::kFewTokens && (tokens + 7) / 8 * touched <= i8::kFewBytes ? 1 : mean <= 64 || tiles <= 56 ? 2 : mean < 1024 ? 0 : 3;
   }
   if (which == 1) {
     i8::FewArgs f;
@@ -1006,17 +1149,12 @@ extern "C" int fmoe_int8_gemm(const int8_t* a, int64_t a_stride, const float* a_
   CUtensorMap map_a, map_w;
   int rc = i8::make_map(&map_a, a, 1, R, K, a_stride, R * a_stride, i8::kBM, 2, "A");
   if (rc != 0) return rc;
-  rc = i8::make_map(&map_w, w, E, N, K, w_stride, E == 1 ? N * w_stride : w_expert_stride, swiglu ? 128 : i8::kBN, 3, "W");
+  rc = i8::make_map(&map_w, w, E, N, K, w_stride, E == 1 ? N * w_stride : w_expert_stride,
+                    swiglu || which == 3 ? 128 : i8::kBN, 3, "W");
   if (rc != 0) return rc;
-  const int64_t max_tiles = ((R + i8::kBM - 1) / i8::kBM + E - 1) * g.n_blocks;
-  const int grid = static_cast<int>(max_tiles < g_gemm_sms ? max_tiles : g_gemm_sms);
-  const size_t smem = 1024 + static_cast<size_t>(i8::kStages) * i8::kStageBytes + 256 + i8::kEpiStageBytes +
-                      sizeof(int) * (E + 2);
-  const int smem_most = 1024 + i8::kStages * i8::kStageBytes + 256 + i8::kEpiStageBytes +
-                        static_cast<int>(sizeof(int)) * (i8::kMaxExperts + 2);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   FMOE_DISPATCH_DTYPE(out_dtype, DT, {
-    FMOE_CUDA(cudaFuncSetAttribute(i8::int8_gemm_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_most));
-    i8::int8_gemm_kernel<DT><<<grid, i8::kTileThreads, smem, static_cast<cudaStream_t>(stream)>>>(map_a, map_w, g);
+    rc = which == 3 ? i8::launch_tiles<DT, true>(map_a, map_w, g, st) : i8::launch_tiles<DT, false>(map_a, map_w, g, st);
   });
-  return check_launch("int8_gemm_kernel");
+  return rc;
 }

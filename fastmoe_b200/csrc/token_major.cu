@@ -499,7 +499,7 @@ extern "C" int fmoe_tune(const char* key, int value) {
     FMOE_REQUIRE(value >= -1 && value <= 1, FMOE_ERR_ARG, "fmoe_tune: gemm_tokens_as_n is -1 (auto), 0 or 1");
     g_gemm_tokens_as_n = value;
   } else if (k == "int8_few_rows") {
-    FMOE_REQUIRE(value >= -1 && value <= 2, FMOE_ERR_ARG, "fmoe_tune: int8_few_rows is -1 (auto), 0, 1 or 2");
+    FMOE_REQUIRE(value >= -1 && value <= 3, FMOE_ERR_ARG, "fmoe_tune: int8_few_rows is -1 (auto) to 3");
     g_int8_few_rows = value;
   } else if (k == "gather_pdl") {
     g_gather_pdl = value != 0;

@@ -136,7 +136,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.
     _check(x, weight, None, eps)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _RmsNorm.apply(x, None, weight, eps)
-    return _forward(_rows(x), None, weight.contiguous(), eps, True, False, False)[0].view(x.shape)
+    return _shaped(_forward(_rows(x), None, weight.contiguous(), eps, True, False, False)[0], x.shape)
 
 
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6):
@@ -149,7 +149,7 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
     if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or weight.requires_grad):
         return _RmsNorm.apply(x, residual, weight, eps)
     y, stream, _, _ = _forward(_rows(x), _rows(residual), weight.contiguous(), eps, True, False, False)
-    return y.view(x.shape), stream.view(x.shape)
+    return _shaped(y, x.shape), _shaped(stream, x.shape)
 
 
 def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
@@ -165,4 +165,5 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
         raise ValueError("rms_norm_int8 has no gradient: call it under torch.no_grad(), or use rms_norm / add_rms_norm")
     y, stream, _, q = _forward(_rows(x), None if residual is None else _rows(residual), weight.contiguous(), eps, with_y,
                                False, True)  # fmt: skip
-    return NormInt8(q, None if stream is None else stream.view(x.shape), None if y is None else y.view(x.shape))
+    shape = x.shape
+    return NormInt8(q, None if stream is None else _shaped(stream, shape), None if y is None else _shaped(y, shape))
