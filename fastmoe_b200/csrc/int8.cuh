@@ -10,6 +10,22 @@
 
 namespace fmoe {
 
+// Quotients by a run-time constant, as a multiplication: n / d = n * (2^s / d + 1) / 2^s for n < 2^31,
+// with s = 31 + ceil(log2 d) (the excess of the factor, below 2^-s each, adds less than 1 / d).
+struct FastDiv {
+  uint32_t mul = 0, shift = 0;
+  int d = 1;
+  explicit FastDiv(int64_t divisor) : d(static_cast<int>(divisor)) {
+    uint32_t log = 0;
+    while ((1ll << log) < divisor) ++log;
+    shift = 31 + log;
+    mul = static_cast<uint32_t>((1ull << shift) / static_cast<uint64_t>(divisor) + 1);
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul) >> shift);
+  }
+};
+
 #ifdef __CUDACC__
 
 constexpr uint32_t kInfBits = 0x7f800000u;
@@ -17,6 +33,13 @@ constexpr uint32_t kInfBits = 0x7f800000u;
 // Largest magnitude of a run as the bit pattern of |v|: unsigned order is the order of the
 // magnitudes, with infinity and NaN above every finite value, so a maximum never loses a NaN.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// Larger of `top` and |v|, NaN if either is.
+__device__ __forceinline__ float max_abs(float top, float v) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(top), "f"(fabsf(v)));
+  return m;
+}
 
 // Adding this to |t| < 2^22 rounds t to a whole number (nearest, ties to even) and leaves that number's
 // two's complement in the low bits of the sum. Conversion instructions run at an eighth of the rate of

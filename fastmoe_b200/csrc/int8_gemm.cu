@@ -1045,7 +1045,7 @@ static int launch_tiles(const CUtensorMap& map_a, const CUtensorMap& map_w, cons
 
 }  // namespace i8
 
-int g_int8_few_rows = -1;  // fmoe_tune "int8_few_rows": 1 / 0 forces the kernel, -1 = by the sizes
+int g_int8_kernel = -1;  // fmoe_tune "int8_kernel": 0 tiles, 1 few rows, 2 split K, 3 pairs; -1 = by the sizes
 
 }  // namespace fmoe
 
@@ -1096,7 +1096,7 @@ extern "C" int fmoe_int8_gemm(const int8_t* a, int64_t a_stride, const float* a_
   // Which kernel: the host knows the rows and the experts, not how the rows are spread.
   const int64_t mean = (R + E - 1) / E, touched = (R < E ? R : E) * N * K;
   const int64_t tokens = E == 1 ? R : 2 * mean;  // rows that an expert may well have
-  int which = g_int8_few_rows;
+  int which = g_int8_kernel;
   if (which < 0) {
     const int64_t tiles = ((R + i8::kBM - 1) / i8::kBM + (R < E ? R : E) - 1) * g.n_blocks;
     // One pass over the weights for every eight rows of an expert costs the few-rows kernel 2 us per 16 MB

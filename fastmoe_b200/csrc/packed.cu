@@ -51,24 +51,9 @@ __device__ __forceinline__ void dequantise8(uint2 w, float s, float2* f) {
   for (int j = 0; j < 4; ++j) f[j] = mul2(make_float2(t[2 * j], t[2 * j + 1]), s2);
 }
 
-// Quotients by a run-time constant, as a multiplication: n / d = n * (2^s / d + 1) / 2^s for n < 2^31,
-// with s = 31 + ceil(log2 d) (the excess of the factor, below 2^-s each, adds less than 1 / d).
-struct FastDiv {
-  uint32_t mul = 0, shift = 0;
-  int d = 1;
-  explicit FastDiv(int64_t divisor) : d(static_cast<int>(divisor)) {
-    uint32_t log = 0;
-    while ((1ll << log) < divisor) ++log;
-    shift = 31 + log;
-    mul = static_cast<uint32_t>((1ull << shift) / static_cast<uint64_t>(divisor) + 1);
-  }
-  __device__ __forceinline__ int div(int n) const {
-    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul) >> shift);
-  }
-};
-
-// Eight lanes share a group, sixteen columns each.
-template <int DT>
+// Eight lanes share a group, sixteen columns each. FULL: whole groups in 16-byte vectors, four to a warp,
+// without the questions that ragged rows ask per vector (the kernel is bound by its instructions).
+template <int DT, bool FULL>
 __global__ void __launch_bounds__(256) pack_kernel(const void* x, int64_t x_stride, int8_t* q, int64_t q_stride,
                                                    float* scale, int total, int D, FastDiv groups, int vec) {
   using E = typename Elem<DT>::type;
@@ -78,7 +63,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* x, int64_t x_stri
   for (int64_t g0 = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x >> 5) * 4; g0 < total;
        g0 += static_cast<int64_t>(gridDim.x) * 32) {
     const int g = static_cast<int>(g0) + ((threadIdx.x >> 3) & 3);
-    const bool live = g < total;
+    const bool live = FULL || g < total;
     const int row_of = live ? groups.div(g) : 0;
     const int64_t row = row_of;
     const int k = g - row_of * groups.d;
@@ -88,6 +73,10 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* x, int64_t x_stri
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 16 / VE; ++i) {
+      if (FULL) {
+        v[i] = ld_stream16(reinterpret_cast<const uint4*>(p + i * VE));
+        continue;
+      }
       v[i] = make_uint4(0, 0, 0, 0);
       if (live && c + i * VE < D) {
         if (vec) {
@@ -105,12 +94,12 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* x, int64_t x_stri
 #pragma unroll
     for (int d = 4; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
     const Quantiser quant(top);
-    if (live && c < q_stride) {  // past D: zeros up to the 16-byte step
+    if (FULL || (live && c < q_stride)) {  // past D: zeros up to the 16-byte step
       float f[16];
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 16 / VE; ++i) unpack16<DT>(v[i], f + i * VE);
-      quant.operator()<16>(f, w);
+      quant.template operator()<16>(f, w);
       st_stream16(reinterpret_cast<uint4*>(q + row * q_stride + c), make_uint4(w[0], w[1], w[2], w[3]));
     }
     if (live && sub == 0) scale[g] = quant.scale();
@@ -215,7 +204,7 @@ using namespace fmoe;
 
 #define FMOE_PACKED_SIZES(name)                                                                             \
   FMOE_REQUIRE(valid_dtype(dtype), FMOE_ERR_ARG, name ": bad dtype");                                       \
-  FMOE_REQUIRE(T >= 0 && D > 0 && T < (1ll << 31) && D < (1ll << 31), FMOE_ERR_ARG, name ": bad sizes");     \
+  FMOE_REQUIRE(T >= 0 && D > 0 && T < (1ll << 31) && D < (1ll << 30), FMOE_ERR_ARG, name ": bad sizes");     \
   if (T == 0) return FMOE_OK;                                                                               \
   FMOE_REQUIRE(T * ((D + 7) / 8) < (1ll << 31) - 1024, FMOE_ERR_UNSUPPORTED, name ": too many values");    \
   FMOE_REQUIRE(q && scale, FMOE_ERR_ARG, name ": null pointer argument");                                   \
@@ -230,9 +219,18 @@ extern "C" int fmoe_pack_activation(const void* x, int64_t x_stride, int8_t* q, 
   FMOE_REQUIRE(T == 1 || x_stride >= D, FMOE_ERR_ARG, "fmoe_pack_activation: the row stride must be at least D");
   const int groups = packed_groups(D);
   const int vec = D % 8 == 0 && aligned_to(x, 16) && x_stride * dtype_size(dtype) % 16 == 0;
-  FMOE_DISPATCH_DTYPE(dtype, DT, pack_kernel<DT><<<stream_grid((T * groups + 31) / 32), 256, 0,
-                                                   static_cast<cudaStream_t>(stream)>>>(x, x_stride, q, q_stride, scale,
-                                                                                        static_cast<int>(T * groups), static_cast<int>(D), FastDiv(groups), vec));
+  const int64_t total = T * groups;
+  const unsigned grid = stream_grid((total + 31) / 32);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool full = vec && D % kGroup == 0 && total % 4 == 0;
+  FMOE_DISPATCH_DTYPE(dtype, DT, {
+    if (full)
+      pack_kernel<DT, true><<<grid, 256, 0, st>>>(x, x_stride, q, q_stride, scale, static_cast<int>(total),
+                                                  static_cast<int>(D), FastDiv(groups), vec);
+    else
+      pack_kernel<DT, false><<<grid, 256, 0, st>>>(x, x_stride, q, q_stride, scale, static_cast<int>(total),
+                                                   static_cast<int>(D), FastDiv(groups), vec);
+  });
   return check_launch("pack_kernel");
 }
 

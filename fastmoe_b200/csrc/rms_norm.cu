@@ -232,7 +232,8 @@ constexpr int row_threads(int elements) { return elements > 8 ? 512 : 1024; }
 // VPT vectors of it in registers, as they lie in memory: what is unpacked twice costs fewer cycles
 // than the CTAs that 32 fp32 registers a thread would keep off the SM.
 template <int DT, int CUT, int VPT, bool WARP, bool NORM>
-__global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::kElems)) row_kernel(const RowArgs a) {
+__global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::kElems),
+                                  !WARP && NORM && CUT == kShifted && DT != FMOE_F32 && VPT == 4 ? 2 : 1) row_kernel(const RowArgs a) {
   __shared__ double part_sum[32];
   __shared__ uint32_t part_max[32];
   constexpr int VE = Vec<DT, CUT>::kElems;
@@ -305,10 +306,19 @@ __global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::k
     if constexpr (NORM) {
       float w[VE];
       load_weight<DT, CUT>(a.w, a.w_f32, first + i * step, D, w);
+      if constexpr (VE > 1) {  // two to an instruction
 #pragma unroll
-      for (int j = 0; j < VE; ++j) f[j] = f[j] * rstd * w[j];
+        for (int j = 0; j < VE; j += 2) {
+          const float2 y = mul2(mul2(make_float2(f[j], f[j + 1]), make_float2(rstd, rstd)), make_float2(w[j], w[j + 1]));
+          f[j] = y.x;
+          f[j + 1] = y.y;
+        }
+      } else {
+        f[0] = f[0] * rstd * w[0];
+      }
     }
   };
+  float top_y = 0.f;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int e = first + i * step;
@@ -323,13 +333,14 @@ __global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::k
         }
         // elements outside the row are zeros, or NaN where the row is not finite
 #pragma unroll
-        for (int j = 0; j < VE; ++j) top = max(top, abs_bits(f[j]));
+        for (int j = 0; j < VE; ++j) top_y = max_abs(top_y, f[j]);
       } else {
         top = sv[i].top(top);
       }
     }
   }
   if (a.q == nullptr) return;
+  if constexpr (NORM) top = abs_bits(top_y);
   const Quantiser quant(row_max<WARP>(top, part_max));
   int8_t* q = a.q + row * a.q_stride;
 #pragma unroll
@@ -649,24 +660,32 @@ __global__ void __launch_bounds__(32 * kDwWarps) rms_dw_kernel(const float* part
 // ---- 8-bit rows back to floating point --------------------------------------------------------
 template <int DT>
 __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* q, int64_t q_stride, const float* scale, void* out,
-                                                         int64_t T, int64_t D, int vec) {
+                                                         int total, int D, FastDiv per_row, int vec) {
   using E = typename Elem<DT>::type;
   constexpr int VE = Elem<DT>::kVec;
-  const int64_t per_row = (D + VE - 1) / VE;
-  const int64_t total = T * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t row = i / per_row, c = (i - row * per_row) * VE;
+    const int row_of = per_row.div(static_cast<int>(i)), c = (static_cast<int>(i) - row_of * per_row.d) * VE;
+    const int64_t row = row_of;
     const float s = scale[row];
     const int8_t* p = q + row * q_stride + c;
     E* o = static_cast<E*>(out) + row * D + c;
-    float f[VE];
     if (vec) {
+      float f[VE];
+      if constexpr (VE == 8) {
+        const uint2 w = *reinterpret_cast<const uint2*>(p);
+        unpack_int8(w.x, f);
+        unpack_int8(w.y, f + 4);
+      } else {
+        unpack_int8(*reinterpret_cast<const uint32_t*>(p), f);
+      }
 #pragma unroll
-      for (int j = 0; j < VE; j += 4) unpack_int8(*reinterpret_cast<const uint32_t*>(p + j), f + j);
-#pragma unroll
-      for (int j = 0; j < VE; ++j) f[j] *= s;
-      *reinterpret_cast<uint4*>(o) = pack16<DT>(f);
+      for (int j = 0; j < VE; j += 2) {
+        const float2 y = mul2(make_float2(f[j], f[j + 1]), make_float2(s, s));
+        f[j] = y.x;
+        f[j + 1] = y.y;
+      }
+      st_stream16(reinterpret_cast<uint4*>(o), pack16<DT>(f));
     } else {
       for (int j = 0; j < VE && c + j < D; ++j) o[j] = from_float<DT>(static_cast<float>(p[j]) * s);
     }
@@ -803,7 +822,7 @@ extern "C" int fmoe_rms_norm(const void* x, int64_t x_stride, const void* residu
   FMOE_RANGE("fmoe_rms_norm");
   FMOE_REQUIRE(valid_dtype(dtype) && (w_dtype == dtype || w_dtype == FMOE_F32), FMOE_ERR_ARG,
                "fmoe_rms_norm: bad dtype (the weight is fp32 or of the rows' type)");
-  FMOE_REQUIRE(T >= 0 && D > 0 && T < (1ll << 31) && D < (1ll << 31), FMOE_ERR_ARG, "fmoe_rms_norm: bad sizes");
+  FMOE_REQUIRE(T >= 0 && D > 0 && T < (1ll << 31) && D < (1ll << 30), FMOE_ERR_ARG, "fmoe_rms_norm: bad sizes");
   FMOE_REQUIRE(eps >= 0.0, FMOE_ERR_ARG, "fmoe_rms_norm: eps must not be negative");
   if (T == 0) return FMOE_OK;
   FMOE_REQUIRE(x && w && (y || q), FMOE_ERR_ARG, "fmoe_rms_norm: null pointer argument");
@@ -832,7 +851,7 @@ extern "C" int fmoe_quantize_rows(const void* x, int64_t x_stride, int8_t* q, in
                                   int64_t D, int dtype, void* stream) {
   FMOE_RANGE("fmoe_quantize_rows");
   FMOE_REQUIRE(valid_dtype(dtype), FMOE_ERR_ARG, "fmoe_quantize_rows: bad dtype");
-  FMOE_REQUIRE(T >= 0 && D > 0 && T < (1ll << 31) && D < (1ll << 31), FMOE_ERR_ARG, "fmoe_quantize_rows: bad sizes");
+  FMOE_REQUIRE(T >= 0 && D > 0 && T < (1ll << 31) && D < (1ll << 30), FMOE_ERR_ARG, "fmoe_quantize_rows: bad sizes");
   if (T == 0) return FMOE_OK;
   FMOE_REQUIRE(x && q && q_scale, FMOE_ERR_ARG, "fmoe_quantize_rows: null pointer argument");
   FMOE_REQUIRE(T == 1 || x_stride >= D, FMOE_ERR_ARG, "fmoe_quantize_rows: the row stride must be at least D");
@@ -852,17 +871,19 @@ extern "C" int fmoe_dequantize_rows(const int8_t* q, int64_t q_stride, const flo
                                     int dtype, void* stream) {
   FMOE_RANGE("fmoe_dequantize_rows");
   FMOE_REQUIRE(valid_dtype(dtype), FMOE_ERR_ARG, "fmoe_dequantize_rows: bad dtype");
-  FMOE_REQUIRE(T >= 0 && D > 0 && T < (1ll << 31) && D < (1ll << 31), FMOE_ERR_ARG, "fmoe_dequantize_rows: bad sizes");
+  FMOE_REQUIRE(T >= 0 && D > 0 && T < (1ll << 31) && D < (1ll << 30), FMOE_ERR_ARG, "fmoe_dequantize_rows: bad sizes");
   if (T == 0) return FMOE_OK;
   FMOE_REQUIRE(q && q_scale && out, FMOE_ERR_ARG, "fmoe_dequantize_rows: null pointer argument");
   FMOE_REQUIRE(T == 1 || q_stride >= D, FMOE_ERR_ARG, "fmoe_dequantize_rows: the row stride must be at least D");
   const int ve = 16 / dtype_size(dtype);
-  const int vec = D % ve == 0 && q_stride % 4 == 0 && aligned_to(q, 4) && aligned_to(out, 16);
-  const int64_t total = T * ((D + ve - 1) / ve);
+  const int vec = D % ve == 0 && q_stride % ve == 0 && aligned_to(q, ve) && aligned_to(out, 16);
+  const int64_t per_row = (D + ve - 1) / ve, total = T * per_row;
+  FMOE_REQUIRE(total < (1ll << 31) - 1024, FMOE_ERR_UNSUPPORTED, "fmoe_dequantize_rows: too many values");
   const int64_t want = (total + 255) / 256, most = 16 * kNumSMs;
   const unsigned grid = static_cast<unsigned>(want < most ? want : most);
   FMOE_DISPATCH_DTYPE(dtype, DT, dequantize_kernel<DT><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
-                                     q, q_stride, q_scale, out, T, D, vec));
+                                     q, q_stride, q_scale, out, static_cast<int>(total), static_cast<int>(D),
+                                     FastDiv(per_row), vec));
   return check_launch("dequantize_kernel");
 }
 
@@ -877,7 +898,7 @@ extern "C" int fmoe_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* 
   FMOE_RANGE("fmoe_rms_norm_bwd");
   FMOE_REQUIRE(valid_dtype(dtype) && (w_dtype == dtype || w_dtype == FMOE_F32), FMOE_ERR_ARG,
                "fmoe_rms_norm_bwd: bad dtype (the weight is fp32 or of the rows' type)");
-  FMOE_REQUIRE(T >= 0 && D > 0 && T < (1ll << 31) && D < (1ll << 31), FMOE_ERR_ARG, "fmoe_rms_norm_bwd: bad sizes");
+  FMOE_REQUIRE(T >= 0 && D > 0 && T < (1ll << 31) && D < (1ll << 30), FMOE_ERR_ARG, "fmoe_rms_norm_bwd: bad sizes");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (T == 0) {  // no rows: the weight's gradient is zero
     if (dw != nullptr) FMOE_CUDA(cudaMemsetAsync(dw, 0, static_cast<size_t>(D) * dtype_size(w_dtype), st));

@@ -23,7 +23,7 @@ static int g_bwd_ctas_per_sm = 3;
 static int g_gather_pdl = 1;  // launch the gather kernels as programmatic dependents of their predecessor
 int g_host_chunks = 1;  // column slices of fmoe_combine_host (host_api.cu); 0 = choose from the sizes
 extern int g_gemm_sms, g_gemm_skip_loads, g_gemm_spin_limit, g_gemm_prefetch, g_gemm_tokens_as_n;  // grouped_gemm.cu
-extern int g_int8_few_rows;  // int8_gemm.cu
+extern int g_int8_kernel;  // int8_gemm.cu
 extern int g_peer_ctas_per_sm;  // ep_fused.cu
 extern int g_plan_rows_per_thread;  // combine_plan.cu
 
@@ -498,9 +498,9 @@ extern "C" int fmoe_tune(const char* key, int value) {
   } else if (k == "gemm_tokens_as_n") {
     FMOE_REQUIRE(value >= -1 && value <= 1, FMOE_ERR_ARG, "fmoe_tune: gemm_tokens_as_n is -1 (auto), 0 or 1");
     g_gemm_tokens_as_n = value;
-  } else if (k == "int8_few_rows") {
-    FMOE_REQUIRE(value >= -1 && value <= 3, FMOE_ERR_ARG, "fmoe_tune: int8_few_rows is -1 (auto) to 3");
-    g_int8_few_rows = value;
+  } else if (k == "int8_kernel") {
+    FMOE_REQUIRE(value >= -1 && value <= 3, FMOE_ERR_ARG, "fmoe_tune: int8_kernel is -1 (auto) to 3");
+    g_int8_kernel = value;
   } else if (k == "gather_pdl") {
     g_gather_pdl = value != 0;
   } else if (k == "plan_rows_per_thread") {

@@ -17,7 +17,6 @@ alike: there is no library fallback.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from . import checkpoint, ops
@@ -221,8 +220,13 @@ class _PackedFFN(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_out):
+        if torch.is_grad_enabled():  # create_graph
+            with torch.no_grad():
+                grads = _PackedFFN.backward(ctx, grad_out)
+            return tuple(None if g is None else
+                         ops._NoSecondDerivative.apply(g, "an FFN with packed activations", grad_out, *ctx.saved_tensors[4:6])
+                         for g in grads)  # fmt: skip
         q, scale, xq, xscale, w1, w2, offsets, counts, row_map = ctx.saved_tensors
         pre_shape, x_shape = ctx.shapes
         if row_map is not None:

@@ -17,7 +17,6 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from . import ops
@@ -59,10 +58,12 @@ def _check(x, weight, residual, eps):
         raise ValueError(f"eps must not be negative, got {eps}")
 
 
-def _forward(x2, r2, weight, eps, want_y, want_rstd, want_q):
-    """One launch over [T, D] rows; returns (y, stream, rstd, Int8Rows)."""
-    T, D = shape = x2.shape
-    dtype = _DTYPES[x2.dtype]
+def _forward(x, residual, weight, eps, want_y, want_rstd, want_q):
+    """One launch over the rows of x; returns (y, stream, rstd, Int8Rows), y and stream in x's shape."""
+    x2 = _rows(x)
+    r2 = None if residual is None else _rows(residual)
+    T, D = x2.shape
+    shape = x.shape
     y = x2.new_empty(shape) if want_y else None
     stream = x2.new_empty(shape) if r2 is not None else None
     rstd = x2.new_empty((T,), dtype=torch.float32) if want_rstd else None
@@ -72,43 +73,10 @@ def _forward(x2, r2, weight, eps, want_y, want_rstd, want_q):
         0 if r2 is None else r2.stride(0), weight.data_ptr(), _DTYPES[weight.dtype],
         None if y is None else y.data_ptr(), None if stream is None else stream.data_ptr(),
         None if rstd is None else rstd.data_ptr(), None if rows is None else rows.q.data_ptr(),
-        0 if rows is None else rows.q.stride(0), None if rows is None else rows.scale.data_ptr(), T, D, eps, dtype,
+        0 if rows is None else rows.q.stride(0), None if rows is None else rows.scale.data_ptr(), T, D, eps,
+        _DTYPES[x2.dtype],
     )  # fmt: skip
     return y, stream, rstd, rows
-
-
-def _shaped(t, shape):
-    return t if t.shape == shape else t.view(shape)
-
-
-def _rms_backward(ctx, dy, dstream=None):
-    if dy is None:  # the normed rows were not used: the stream's gradient passes through
-        return dstream, dstream if ctx.needs_input_grad[1] else None, None, None
-    s, rstd, weight = ctx.saved_tensors
-    T, D = s.shape
-    dy2 = _rows(dy if dy.dtype == s.dtype else dy.to(s.dtype))
-    ds2 = None
-    if dstream is not None:
-        ds2 = _rows(dstream if dstream.dtype == s.dtype else dstream.to(s.dtype))
-    dx = s.new_empty((T, D))
-    dw = scratch = None
-    nbytes = 0
-    if ctx.needs_input_grad[2]:
-        dw = weight.new_empty(weight.shape)
-        nbytes = _lib.lib().fmoe_rms_norm_bwd_bytes(T, D)
-        scratch = s.new_empty((nbytes,), dtype=torch.uint8)
-    ops._launch(
-        s.get_device(), "fmoe_rms_norm_bwd", 1 if dw is None else 2, dy2.data_ptr(), dy2.stride(0),
-        None if ds2 is None else ds2.data_ptr(), 0 if ds2 is None else ds2.stride(0), s.data_ptr(), s.stride(0),
-        rstd.data_ptr(), weight.data_ptr(), _DTYPES[weight.dtype], dx.data_ptr(),
-        None if dw is None else dw.data_ptr(), None if scratch is None else scratch.data_ptr(), nbytes, T, D,
-        _DTYPES[s.dtype],
-    )  # fmt: skip
-    dx = _shaped(dx, ctx.shape)
-    return dx, dx if ctx.needs_input_grad[1] else None, dw, None
-
-
-_rms_backward_once = once_differentiable(_rms_backward)
 
 
 class _RmsNorm(torch.autograd.Function):
@@ -116,18 +84,41 @@ class _RmsNorm(torch.autograd.Function):
     def forward(ctx, x, residual, weight, eps):
         ctx.set_materialize_grads(False)
         weight = weight.contiguous()
-        x2 = _rows(x)
-        y, stream, rstd, _ = _forward(x2, None if residual is None else _rows(residual), weight, eps, True, True, False)
-        ctx.save_for_backward(x2 if stream is None else stream, rstd, weight)
-        ctx.shape = shape = x.shape
-        if stream is None:
-            return _shaped(y, shape)
-        return _shaped(y, shape), _shaped(stream, shape)
+        y, stream, rstd, _ = _forward(x, residual, weight, eps, True, True, False)
+        ctx.save_for_backward(x if stream is None else stream, rstd, weight)
+        return y if stream is None else (y, stream)
 
     @staticmethod
-    def backward(ctx, *grads):
-        # there is no second derivative: under create_graph the result is marked so
-        return (_rms_backward_once if torch.is_grad_enabled() else _rms_backward)(ctx, *grads)
+    def backward(ctx, dy, dstream=None):
+        if dy is None:  # the normed rows were not used: the stream's gradient passes through
+            return dstream, dstream if ctx.needs_input_grad[1] else None, None, None
+        stream, rstd, weight = ctx.saved_tensors
+        s = _rows(stream)
+        T, D = s.shape
+        dtype = s.dtype
+        dy2 = _rows(dy if dy.dtype == dtype else dy.to(dtype))
+        ds2 = None
+        if dstream is not None:
+            ds2 = _rows(dstream if dstream.dtype == dtype else dstream.to(dtype))
+        dx = s.new_empty(stream.shape)
+        dw = scratch = None
+        nbytes = 0
+        if ctx.needs_input_grad[2]:
+            dw = weight.new_empty(weight.shape)
+            nbytes = _lib.lib().fmoe_rms_norm_bwd_bytes(T, D)
+            scratch = s.new_empty((nbytes,), dtype=torch.uint8)
+        ops._launch(
+            s.get_device(), "fmoe_rms_norm_bwd", 1 if dw is None else 2, dy2.data_ptr(), dy2.stride(0),
+            None if ds2 is None else ds2.data_ptr(), 0 if ds2 is None else ds2.stride(0), s.data_ptr(), s.stride(0),
+            rstd.data_ptr(), weight.data_ptr(), _DTYPES[weight.dtype], dx.data_ptr(),
+            None if dw is None else dw.data_ptr(), None if scratch is None else scratch.data_ptr(), nbytes, T, D,
+            _DTYPES[dtype],
+        )  # fmt: skip
+        if torch.is_grad_enabled():  # create_graph
+            dx = ops._NoSecondDerivative.apply(dx, "the RMS norm", stream, weight, dy)
+            if dw is not None:
+                dw = ops._NoSecondDerivative.apply(dw, "the RMS norm", stream, weight, dy)
+        return dx, dx if ctx.needs_input_grad[1] else None, dw, None
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
@@ -136,7 +127,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.
     _check(x, weight, None, eps)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _RmsNorm.apply(x, None, weight, eps)
-    return _shaped(_forward(_rows(x), None, weight.contiguous(), eps, True, False, False)[0], x.shape)
+    return _forward(x, None, weight.contiguous(), eps, True, False, False)[0]
 
 
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6):
@@ -148,8 +139,7 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
     _check(x, weight, residual, eps)
     if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or weight.requires_grad):
         return _RmsNorm.apply(x, residual, weight, eps)
-    y, stream, _, _ = _forward(_rows(x), _rows(residual), weight.contiguous(), eps, True, False, False)
-    return _shaped(y, x.shape), _shaped(stream, x.shape)
+    return _forward(x, residual, weight.contiguous(), eps, True, False, False)[:2]
 
 
 def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
@@ -163,7 +153,5 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
         x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)
     ):
         raise ValueError("rms_norm_int8 has no gradient: call it under torch.no_grad(), or use rms_norm / add_rms_norm")
-    y, stream, _, q = _forward(_rows(x), None if residual is None else _rows(residual), weight.contiguous(), eps, with_y,
-                               False, True)  # fmt: skip
-    shape = x.shape
-    return NormInt8(q, None if stream is None else _shaped(stream, shape), None if y is None else _shaped(y, shape))
+    y, stream, _, rows = _forward(x, residual, weight.contiguous(), eps, with_y, False, True)
+    return NormInt8(rows, stream, y)

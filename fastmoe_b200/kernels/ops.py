@@ -315,6 +315,21 @@ def _launch(device: int, fn_name, n_kernels, *args):
     return _lib.call(fn_name, *args, stream)
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    """Passes a gradient through and says what is wrong when that gradient is differentiated again. A
+    backward pass under create_graph hands its results through here together with what they depend on:
+    without it they would count as constants, and a penalty on them would silently have no gradient."""
+
+    @staticmethod
+    def forward(ctx, grad, what, *depends_on):
+        ctx.what = what
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.what} has no second derivative")
+
+
 def _combine_into(expert_tensors, indices, weights, out, metadata, accumulate, mode=None):
     """Runs the combine into `out` ([T, D], any row stride). Returns the plan (or None)."""
     mode = _mode if mode is None else mode

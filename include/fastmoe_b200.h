@@ -69,8 +69,9 @@ const char* fmoe_status_name(int status);
  * "gemm_tokens_as_n" (which of fmoe_grouped_gemm's two forward kernels runs: 1 = the expert's
  * tokens are the MMA's N dimension, in steps of 16 rows; 0 = they are its M dimension, in
  * blocks of 128 rows; -1 = by the average rows per expert, the default),
- * "int8_few_rows" (which kernel fmoe_int8_gemm launches: 1 = the one that streams the weights past a
- * few rows, 0 = the tiled tcgen05 one, -1 = by the average rows per expert, the default),
+ * "int8_kernel" (which kernel fmoe_int8_gemm launches: 0 = tiles of 128 x 256, 1 = weights streamed past a
+ * few rows, 2 = weight rows as the MMA's M with K split over a cluster, 3 = tiles of 256 x 256 by pairs
+ * of CTAs; -1 = by the sizes, the default),
  * "peer_ctas_per_sm" (CTAs per SM of fmoe_permute_peer_fwd when it sends one group of experts
  * beside a running grouped GEMM: default 2; 0 = one CTA per work item, as for a pass over all),
  * "gemm_prefetch" (weight k-blocks of 64 the grouped GEMM asks into L2 ahead of its loads:
@@ -450,8 +451,9 @@ int fmoe_dequantize_rows(const int8_t* q, int64_t q_stride, const float* q_scale
  * rounding to out_dtype. a int8 [R, K], w int8 [E, N, K]: row strides (and w's expert stride) in
  * bytes, multiples of 16, at least K; any R, N and K < 131072 (the bytes from K up to the next
  * multiple of 16 must be readable; what they hold does not matter). C contiguous, [R, N], or [R, N/2] for
- * FMOE_ACT_SWIGLU (gate rows of w first). Rows outside every expert are not touched. E <= 1024. An
- * expert whose range runs past row R is cut off there (FMOE_STATUS_BAD_EXPERT).
+ * FMOE_ACT_SWIGLU (gate rows of w first). The experts' ranges must not overlap; rows outside all of
+ * them are not touched. E <= 1024. An expert whose range runs past row R is cut off there
+ * (FMOE_STATUS_BAD_EXPERT).
  */
 int fmoe_int8_gemm(const int8_t* a, int64_t a_stride, const float* a_scale, const int8_t* w, int64_t w_stride,
                    int64_t w_expert_stride, const float* w_scale, void* c, const int64_t* offsets,

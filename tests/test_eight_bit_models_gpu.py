@@ -84,6 +84,19 @@ def test_packed_ffn(act, with_map):
         assert torch.equal(ffn(x, w1, w2, off, cnt, row_map, covers_all_rows=True, packed=True), plain)
 
 
+def test_packed_ffn_has_no_second_derivative():
+    g = torch.Generator(device=DEV).manual_seed(2)
+    w1, w2 = _randn(g, 1, 512, 256, scale=1 / 16).requires_grad_(True), _randn(g, 1, 256, 256, scale=1 / 16)
+    x = _randn(g, 9, 256).requires_grad_(True)
+    cnt = torch.tensor([9], device=DEV)
+    out = experts.grouped_swiglu_ffn(x, w1, w2, cnt - cnt, cnt, covers_all_rows=True, packed=True)
+    plain = torch.autograd.grad(out.sum(), (x, w1), retain_graph=True)
+    again = torch.autograd.grad(out.sum(), (x, w1), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, again))
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(again[0].float().sum() + w1.float().sum(), w1)
+
+
 def test_packed_ffn_refusals():
     w1 = torch.zeros(2, 512, 256, dtype=BF16, device=DEV, requires_grad=True)
     x = torch.zeros(4, 256, dtype=BF16, device=DEV)

@@ -11,6 +11,18 @@ from fastmoe_b200.kernels.int8 import Int8Rows, Int8Weight
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+KERNELS = {"by the sizes": -1, "tiles": 0, "few rows": 1, "split K": 2, "pairs": 3}
+
+
+@pytest.fixture(params=sorted(KERNELS), autouse=True)
+def kernel(request):
+    """Every test of this file runs with the kernel that the library picks and with each of the four behind
+    fmoe_int8_gemm."""
+    _lib.tune("int8_kernel", KERNELS[request.param])
+    yield request.param
+    _lib.tune("int8_kernel", -1)
+
+
 ACTS = {"none": _lib.ACT_NONE, "swiglu": _lib.ACT_SWIGLU, "gelu": _lib.ACT_GELU}
 
 
@@ -260,7 +272,7 @@ def test_norm_to_experts_together(act, ffn):
 def test_on_a_side_stream_and_in_graphs():
     """Two captured graphs of the same call, replayed on two streams at once, and an eager call between
     them: no memory is shared between calls."""
-    cases = [_case(5, 512, 300, seed=4), _case(300, 512, 300, seed=5)]
+    cases = [_case(5, 512, 300, seed=4), _case(300, 512, 300, seed=5), _case(2100, 256, 300, seed=6)]
     streams, graphs, outs = [torch.cuda.Stream() for _ in cases], [], []
     for (a, w), s in zip(cases, streams):
         int8.int8_linear(a, w)
@@ -280,8 +292,10 @@ def test_on_a_side_stream_and_in_graphs():
         _check(out, _product64(a, w.q, w.scale), "none", torch.bfloat16)
 
 
-def test_waits_that_run_out_are_reported():
+def test_waits_that_run_out_are_reported(kernel):
     """With its producer issuing nothing, the product's bounded waits give up: status bit, no hang."""
+    if kernel == "few rows":
+        return  # it waits for nothing
     a, w = _case(600, 256, 512)
     _lib.tune("gemm_skip_loads", 1)
     _lib.tune("gemm_spin_limit", 2000)

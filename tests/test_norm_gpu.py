@@ -140,6 +140,52 @@ def test_rows_with_strides(D):
     assert out.stream.shape == out.y.shape == x3.shape and out.rows.q.shape == (30, D)
 
 
+@pytest.mark.parametrize("wdtype", [torch.bfloat16, torch.float32])
+def test_a_weight_off_the_16_byte_grid(wdtype):
+    x, r, dy, ds, w = _inputs(20, 513, torch.bfloat16, wdtype)
+    x, r, dy, ds, w = x[:, 1:].contiguous(), r[:, :512], dy[:, :512], ds[:, :512], w[1:]
+    xs, ws = x.clone().requires_grad_(True), w.detach().requires_grad_(True)
+    y, s = norm.add_rms_norm(xs, r, ws, EPS)
+    _check_forward(y.detach(), s.detach(), w)
+    gx, gw = torch.autograd.grad((y, s), (xs, ws), (dy, ds))
+    _check_backward(gx, gw, s.detach(), w, dy, ds)
+
+
+def test_no_second_derivative():
+    x, r, dy, ds, w = _inputs(3, 64, torch.float32)
+    x.requires_grad_(True)
+    y, _ = norm.add_rms_norm(x, r, w, EPS)
+    (gx,) = torch.autograd.grad(y, x, dy, create_graph=True)
+    (plain,) = torch.autograd.grad(norm.add_rms_norm(x, r, w, EPS)[0], x, dy)
+    assert torch.equal(gx, plain)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(gx.sum() + x.sum(), x)
+
+
+def test_a_stream_changed_in_place_is_noticed():
+    x, r, dy, ds, w = _inputs(3, 64, torch.float32)
+    x.requires_grad_(True)
+    for shape in ((3, 64), (1, 3, 64)):
+        y, s = norm.add_rms_norm(x.view(shape), r.view(shape), w, EPS)
+        s.add_(1)
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            torch.autograd.grad(y, x, dy.view(shape))
+
+
+def test_one_tensor_as_both_inputs_and_leaves_that_accumulate():
+    x, _, dy, ds, w = _inputs(5, 96, torch.float32)
+    x.requires_grad_(True)
+    y, s = norm.add_rms_norm(x, x, w, EPS)
+    torch.autograd.backward((y, s), (dy, ds))
+    r = x.detach().clone().requires_grad_(True)
+    x2 = x.detach().clone().requires_grad_(True)
+    y, s = norm.add_rms_norm(x2, r, w, EPS)
+    torch.autograd.backward((y, s), (dy, ds))
+    assert torch.equal(x.grad, 2 * x2.grad) and torch.equal(x2.grad, r.grad)
+    r.grad.add_(1)  # each leaf has a gradient of its own
+    assert not torch.equal(x2.grad, r.grad)
+
+
 def test_rows_of_zeros_and_of_infinities():
     x = torch.randn(6, 300, device=DEV)
     x[1] = 0
