@@ -233,7 +233,7 @@ constexpr int row_threads(int elements) { return elements > 8 ? 512 : 1024; }
 // than the CTAs that 32 fp32 registers a thread would keep off the SM.
 template <int DT, int CUT, int VPT, bool WARP, bool NORM>
 __global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::kElems),
-                                  !WARP && NORM && CUT == kShifted && DT != FMOE_F32 && VPT == 4 ? 2 : 1) row_kernel(const RowArgs a) {
+                                  !WARP && NORM && DT != FMOE_F32 && VPT == 4 ? 2 : 1) row_kernel(const RowArgs a) {
   __shared__ double part_sum[32];
   __shared__ uint32_t part_max[32];
   constexpr int VE = Vec<DT, CUT>::kElems;
