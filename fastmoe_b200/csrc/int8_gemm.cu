@@ -56,6 +56,10 @@ struct Args {
 constexpr uint32_t kIdesc = (2u << 4) | (1u << 7) | (1u << 10) | ((kBN >> 3) << 17) | ((kBM >> 4) << 24);
 constexpr uint32_t kIdescPair = (2u << 4) | (1u << 7) | (1u << 10) | ((kBN >> 3) << 17) | ((2 * kBM >> 4) << 24);
 
+// Programmatic dependent launch: a kernel launched so may start while the one before it in the stream ends;
+// everything it reads or writes comes after this wait.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -505,6 +509,7 @@ __global__ void __launch_bounds__(kFewThreads) int8_few_rows_kernel(const FewArg
   const int K = static_cast<int>(f.K);
   const bool swiglu = a.act == FMOE_ACT_SWIGLU;
 
+  wait_for_previous_kernel();
   for (int e = threadIdx.x; e < a.E; e += kFewThreads) {
     const int64_t n = rows_of(a, e);
     if (a.counts != nullptr && n != a.counts[e] && a.counts[e] > 0 && a.status != nullptr && blockIdx.x == 0)
@@ -738,15 +743,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   int fills = 0;
   bool mma_issued = false;
 
-  // ---- set-up ----------------------------------------------------------------------------
-  for (int e = threadIdx.x; e < a.E; e += kThreads) {
-    const int64_t n = rows_of(a, e);
-    if (a.counts != nullptr && n != a.counts[e] && a.counts[e] > 0 && a.status != nullptr && blockIdx.x == 0)
-      atomicOr(a.status, FMOE_STATUS_BAD_EXPERT);  // rows past the end of A were cut off
-    chunk_prefix[e + 1] = static_cast<int>((n + NB - 1) / NB);
-  }
+  // ---- set-up: barriers and TMEM, which need nobody's results, then the chunk table ------------
   if (threadIdx.x == 0) {
-    chunk_prefix[0] = 0;
     *abort_flag = 0;
     for (int s = 0; s < kS; ++s) {
       mbar_init(&full[s], 1);
@@ -759,6 +757,20 @@ __global__ void __launch_bounds__(kThreads, 2)
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)),
+                 "n"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  wait_for_previous_kernel();
+  for (int e = threadIdx.x; e < a.E; e += kThreads) {
+    const int64_t n = rows_of(a, e);
+    if (a.counts != nullptr && n != a.counts[e] && a.counts[e] > 0 && a.status != nullptr && blockIdx.x == 0)
+      atomicOr(a.status, FMOE_STATUS_BAD_EXPERT);  // rows past the end of A were cut off
+    chunk_prefix[e + 1] = static_cast<int>((n + NB - 1) / NB);
+  }
+  if (threadIdx.x == 0) chunk_prefix[0] = 0;
   __syncthreads();
   if (warp == 0) {
     int carry = 0;
@@ -773,12 +785,6 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (e < a.E) chunk_prefix[e + 1] = carry + v;
       carry += __shfl_sync(0xffffffffu, v, 31);
     }
-  }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_slot)),
-                 "n"(kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -994,7 +1000,17 @@ static int launch_few(const FewArgs& f, int64_t items, cudaStream_t st) {
   const int smem = static_cast<int>(sizeof(int)) * (f.g.E + 1);
   FMOE_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, int8_few_rows_kernel<DT, NT>, kFewThreads, smem));
   const int64_t most = static_cast<int64_t>(per_sm > 0 ? per_sm : 1) * kNumSMs;
-  int8_few_rows_kernel<DT, NT><<<static_cast<unsigned>(items < most ? items : most), kFewThreads, smem, st>>>(f);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(static_cast<unsigned>(items < most ? items : most));
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  FMOE_CUDA(cudaLaunchKernelEx(&cfg, int8_few_rows_kernel<DT, NT>, f));
   return check_launch("int8_few_rows_kernel");
 }
 
@@ -1005,17 +1021,19 @@ static int launch_tn(const CUtensorMap& map_t, const CUtensorMap& map_w, const T
   FMOE_CUDA(cudaFuncSetAttribute(int8_tn_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  kFixed + static_cast<int>(sizeof(int)) * (kMaxExperts + 2)));
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   const int64_t most = 2 * static_cast<int64_t>(g_gemm_sms);
   cfg.gridDim = dim3(static_cast<unsigned>(f.splits > 1 ? items * f.splits : items < most ? items : most));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = f.splits;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = f.splits;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = f.splits > 1 ? 1 : 0;
+  cfg.numAttrs = f.splits > 1 ? 2 : 1;
   FMOE_CUDA(cudaLaunchKernelEx(&cfg, int8_tn_kernel<NB>, map_t, map_w, f));
   return check_launch("int8_tn_kernel");
 }

@@ -233,11 +233,13 @@ constexpr int row_threads(int elements) { return elements > 8 ? 512 : 1024; }
 // than the CTAs that 32 fp32 registers a thread would keep off the SM.
 template <int DT, int CUT, int VPT, bool WARP, bool NORM>
 __global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::kElems),
-                                  !WARP && NORM && DT != FMOE_F32 && VPT == 4 ? 2 : 1) row_kernel(const RowArgs a) {
+                                  !WARP && NORM && DT != FMOE_F32 && VPT == 4 ? 2 : 0) row_kernel(const RowArgs a) {
   __shared__ double part_sum[32];
   __shared__ uint32_t part_max[32];
   constexpr int VE = Vec<DT, CUT>::kElems;
   const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y : blockIdx.x;
+  // the product that reads these rows may set itself up meanwhile; it waits for this grid to end
+  if (a.q != nullptr) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (row >= a.T) return;  // WARP only: no barrier follows
   const int tid = threadIdx.x, nthr = WARP ? 32 : blockDim.x;
   const int D = static_cast<int>(a.D);
