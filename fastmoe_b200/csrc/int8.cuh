@@ -127,6 +127,36 @@ struct Quantiser {
       if (side > 0.f || (side == 0.f && (__float_as_uint(s) & 1u))) s += sign;
     }
   }
+  // Values that come straight from a 16-bit type. With significands of 11 bits or fewer, a = b 2^x and
+  // v = c 2^y, a quotient that is not on a border is |254 c - odd b 2^s| / (2 b 2^s) >= |t| / (254 * 2047)
+  // = 1.9e-6 |t| away from it: more than a factor that is too large by 2.4e-7 to 7.2e-7 moves it. That leaves the
+  // exact ties, 254 c = odd b 2^s: either v = a / 2, where 63.5 belongs to 64 and the excess takes it
+  // there, or b is a multiple of 127, which one largest magnitude in 128 is: only then each value is
+  // looked at as any fp32 value is.
+  template <int N>
+  __device__ __forceinline__ void from16(const float* v, uint32_t* words) const {
+    const uint32_t significand = (__float_as_uint(top) & 0x7fffffu) | 0x800000u;
+    if (!fine || significand % 127u == 0u) return this->template operator()<N>(v, words);
+    const float more = inv * (1.f + 0x1p-21f);
+    float s[N];
+    if constexpr (N == 1) {
+      s[0] = fmaf(v[0], more, kRounder);
+      words[0] = __float_as_uint(s[0]) & 255u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; j += 2) {
+        const float2 t = fma2(make_float2(v[j], v[j + 1]), make_float2(more, more), make_float2(kRounder, kRounder));
+        s[j] = t.x;
+        s[j + 1] = t.y;
+      }
+#pragma unroll
+      for (int j = 0; j < N; j += 4) {
+        const uint32_t lo = __byte_perm(__float_as_uint(s[j]), __float_as_uint(s[j + 1]), 0x0040);
+        const uint32_t hi = __byte_perm(__float_as_uint(s[j + 2]), __float_as_uint(s[j + 3]), 0x0040);
+        words[j / 4] = __byte_perm(lo, hi, 0x5410);
+      }
+    }
+  }
   // N values: words[i] holds q of v[4 i .. 4 i + 3] (N = 1: of v[0], in the low byte). The budget is
   // tight: three bytes of DRAM traffic per 16-bit value leave eight instructions for it, so the
   // arithmetic goes in pairs.
@@ -176,19 +206,22 @@ struct Quantiser {
   }
 };
 
-// Bits of the largest |v| of a 16-byte vector of DT (see abs_bits), NaN if one is NaN.
+// Largest |v| over 16-byte vectors of DT as they lie in memory: a run keeps a word (for 16-bit types one
+// maximum in each half; unsigned order again) and ends with top_bits.
 template <int DT>
 __device__ __forceinline__ uint32_t vec_top(const uint4& v, uint32_t top) {
-  if constexpr (DT == FMOE_F32) {
+  if constexpr (DT == FMOE_F32)
     return max(max(top, max(v.x & 0x7fffffffu, v.y & 0x7fffffffu)), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
-  } else {  // two 16-bit magnitudes to a word: unsigned order again, in each half
-    const uint32_t m = __vimax3_u16x2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu,
-                                      __vimax3_u16x2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu, 0u));
-    const uint16_t b = static_cast<uint16_t>(max(m & 0xffffu, m >> 16));
-    float f;
-    if constexpr (DT == FMOE_BF16) f = __uint_as_float(static_cast<uint32_t>(b) << 16);
-    else f = __half2float(__ushort_as_half(b));
-    return max(top, abs_bits(f));
+  else
+    return __vimax3_u16x2(__vimax3_u16x2(top, v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), v.z & 0x7fff7fffu, v.w & 0x7fff7fffu);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t top_bits(uint32_t top) {
+  if constexpr (DT == FMOE_F32) {
+    return top;
+  } else {
+    const uint32_t b = max(top & 0xffffu, top >> 16);
+    return DT == FMOE_BF16 ? b << 16 : abs_bits(__half2float(__ushort_as_half(static_cast<uint16_t>(b))));
   }
 }
 

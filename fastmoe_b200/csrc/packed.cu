@@ -91,6 +91,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* x, int64_t x_stri
     }
 #pragma unroll
     for (int i = 0; i < 16 / VE; ++i) top = vec_top<DT>(v[i], top);
+    top = top_bits<DT>(top);
 #pragma unroll
     for (int d = 4; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
     const Quantiser quant(top);
@@ -99,7 +100,8 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* x, int64_t x_stri
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 16 / VE; ++i) unpack16<DT>(v[i], f + i * VE);
-      quant.template operator()<16>(f, w);
+      if constexpr (DT == FMOE_F32) quant.template operator()<16>(f, w);
+      else quant.template from16<16>(f, w);
       st_stream16(reinterpret_cast<uint4*>(q + row * q_stride + c), make_uint4(w[0], w[1], w[2], w[3]));
     }
     if (live && sub == 0) scale[g] = quant.scale();

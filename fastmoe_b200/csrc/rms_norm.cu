@@ -118,6 +118,7 @@ struct Vec {
     else store_partial<DT>(row, e, D, v);
   }
   __device__ __forceinline__ uint32_t top(uint32_t t) const { return vec_top<DT>(v, t); }
+  __device__ __forceinline__ static uint32_t bits(uint32_t t) { return top_bits<DT>(t); }
 };
 template <int DT>
 struct Vec<DT, kSingle> {
@@ -131,6 +132,7 @@ struct Vec<DT, kSingle> {
   __device__ __forceinline__ void set(const float* f) { v = from_float<DT>(f[0]); }
   __device__ __forceinline__ void store(E* row, int e, int) const { row[e] = v; }
   __device__ __forceinline__ uint32_t top(uint32_t t) const { return max(t, abs_bits(to_float<DT>(v))); }
+  __device__ __forceinline__ static uint32_t bits(uint32_t t) { return t; }
 };
 
 // Weights e .. e + VE - 1, fp32 or of the rows' type, as floats; zeros outside the row. The weight
@@ -343,6 +345,7 @@ __global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::k
   }
   if (a.q == nullptr) return;
   if constexpr (NORM) top = abs_bits(top_y);
+  else top = Vec<DT, CUT>::bits(top);
   const Quantiser quant(row_max<WARP>(top, part_max));
   int8_t* q = a.q + row * a.q_stride;
 #pragma unroll
@@ -352,7 +355,8 @@ __global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::k
       float f[VE];
       uint32_t words[(VE + 3) / 4];
       value(i, f);
-      quant.template operator()<VE>(f, words);
+      if constexpr (NORM || DT == FMOE_F32) quant.template operator()<VE>(f, words);
+      else quant.template from16<VE>(f, words);
       store_int8<VE, CUT>(q, e, D, words);
     }
   }
@@ -407,7 +411,8 @@ __global__ void __launch_bounds__(1024) row_loop_kernel(const RowArgs a) {
   for (int c = threadIdx.x; c < D; c += blockDim.x) {
     const float f = value(c);
     uint32_t word;
-    quant.operator()<1>(&f, &word);
+    if constexpr (NORM || DT == FMOE_F32) quant.operator()<1>(&f, &word);
+    else quant.from16<1>(&f, &word);
     q[c] = static_cast<int8_t>(word);
   }
   const int pad = static_cast<int>((16 - (a.D & 15)) & 15);

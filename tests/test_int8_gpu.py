@@ -165,6 +165,32 @@ def test_operands_off_the_16_byte_grid_and_with_strides():
     _check(int8.int8_linear(a, wt, torch.float32), _product64(a, wt.q, wt.scale), "none", torch.float32)
 
 
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 8), (torch.float16, 11)])
+def test_every_quotient_of_16_bit_values(kernel, dtype, bits):
+    """A row for each significand of the largest magnitude, with all significands of the values in the nine
+    binades below it: among them every exact tie."""
+    if kernel != "by the sizes":
+        return  # there is no product in it
+    one = 2 ** (bits - 1)
+    sig = torch.arange(one, 2 * one, device=DEV, dtype=torch.float32) / one
+    values = torch.cat([sig * 2.0**-e for e in range(9)])
+    x = torch.where(values[None] <= sig[:, None], values[None], -sig[:, None] / 2).to(dtype)
+    x[:, 1::2] *= -1
+    x = torch.cat([sig[:, None].to(dtype), x], 1)
+    assert torch.equal(x.abs().amax(1).float(), sig)
+    for scale in (1.0, 2.0**-5):
+        rows = int8.quantize_rows(x * scale)
+        assert_quantised(rows.q, rows.scale, x * scale)
+    # the same values in groups of 128 columns, each with its row's largest value in front
+    from fastmoe_b200.kernels import checkpoint
+
+    n = (x.shape[1] - 1) // 127 * 127
+    groups = torch.cat([x[:, :1, None].expand(-1, n // 127, 1), x[:, 1 : n + 1].view(one, -1, 127)], 2)
+    p = checkpoint.pack_activation(groups.reshape(one, -1))
+    for k in range(n // 127):
+        assert_quantised(p.q[:, 128 * k : 128 * k + 128], p.scale[:, k], groups[:, k])
+
+
 @pytest.mark.parametrize("K", [1, 33, 640, 7168])
 def test_quantised_operands_end_to_end(K):
     g = _gen(K)
