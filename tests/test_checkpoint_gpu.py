@@ -10,7 +10,8 @@ from fastmoe_b200.kernels import checkpoint
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
-SHAPES = [(1, 1), (1, 128), (2, 2), (3, 30), (5, 127), (4, 129), (7, 256), (33, 1000), (200, 514), (3, 4096), (100, 2056)]
+SHAPES = [(1, 1), (1, 128), (2, 2), (3, 30), (5, 127), (4, 129), (7, 256), (33, 1000), (200, 514), (3, 4096), (100, 2056),
+          (5, 16), (3, 144), (7, 2000), (6, 528)]  # fmt: skip
 
 
 def _x(T, D, dtype, seed=0):
