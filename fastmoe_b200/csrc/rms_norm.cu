@@ -444,8 +444,13 @@ struct RowBwdArgs {
 // vectors of the next row into shared memory slots of its own while it works on this one: with the
 // loads issued row by row into registers two CTAs an SM left HBM idle half of the time between
 // them (16384 x 7168 bf16: 169 us, 5.5 TB/s).
+// CTAs of eight one-warp rows that an SM holds at a time, for the columns of a thread: the grid is this many
+// to an SM, all of them at once (60000 x 200 bf16 34 -> 24 us, 23437 x 512 29 -> 22 us, against four to an SM).
+constexpr int warp_ctas(int columns) { return columns <= 8 ? 3 : 2; }
+
 template <int DT, int CUT, int VPT, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::kElems)) rms_bwd_kernel(const RowBwdArgs a) {
+__global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::kElems),
+                                  WARP ? warp_ctas(VPT * Vec<DT, CUT>::kElems) : 0) rms_bwd_kernel(const RowBwdArgs a) {
   __shared__ float part_sum[2][32];
   extern __shared__ __align__(16) float w_smem[];
   constexpr int VE = Vec<DT, CUT>::kElems;
@@ -471,9 +476,16 @@ __global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::k
         for (int j = 0; j < kWide; ++j) w_smem[p * plane + (i * nthr + tid) * kWide + j] = w[p * kWide + j];
     }
   }  // each thread reads back what it wrote itself: no barrier
+  float w_own[WARP ? VPT : 1][VE];  // a warp's row is short enough for registers
+  if constexpr (WARP) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (first + i * step < D) load_weight<DT, CUT>(a.w, a.w_f32, first + i * step, D, w_own[i]);
+  }
   auto weight = [&](int i, float* w) {
     if constexpr (WARP) {
-      load_weight<DT, CUT>(a.w, a.w_f32, first + i * step, D, w);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) w[j] = w_own[i][j];
     } else if constexpr (VE >= 4) {
 #pragma unroll
       for (int p = 0; p < kPlanes; ++p) {
@@ -489,8 +501,9 @@ __global__ void __launch_bounds__(WARP ? 256 : row_threads(VPT * Vec<DT, CUT>::k
   for (int i = 0; i < VPT; ++i)
 #pragma unroll
     for (int j = 0; j < VE; ++j) dw[i][j] = 0.f;
-  constexpr bool kAhead = !WARP && CUT != kSingle;
-  uint4* slots = reinterpret_cast<uint4*>(w_smem + kPlanes * plane) + tid;  // [3][VPT][nthr], kAhead only
+  constexpr bool kAhead = CUT != kSingle;
+  uint4* slots = reinterpret_cast<uint4*>(w_smem + (WARP ? (D + 3) / 4 * 4 : kPlanes * plane)) +
+                 (WARP ? threadIdx.y * (3 * VPT * 32) : 0) + tid;  // [3][VPT][nthr], kAhead only
   const int64_t row_step = static_cast<int64_t>(gridDim.x) * rows_per_cta;
   auto fetch = [&](int64_t row) {
     if constexpr (kAhead) {
@@ -723,13 +736,16 @@ struct RowGrid {
 
 // How a row is split: a warp per row while a row fits 32 threads, else a CTA. A CTA takes four vectors a
 // thread when there are rows enough to fill the GPU (more loads in flight per thread), one or two
-// when there are not (the latency of a single row falls with the vectors per thread).
+// when there are not (the latency of a single row falls with the vectors per thread). The backward pass
+// of 16-bit rows of up to 256 vectors takes two: it holds three inputs and the dw of eight columns to a
+// vector, and is short of warps at four (14742 x 814 bf16 43 -> 29 us, 11718 x 1024 23 -> 19; fp32 rows,
+// half the columns to a vector, are slower with two, 33 -> 38 us).
 struct RowShape {
   Cut cut;
   bool warp, loop;
   int vpt, threads;
 };
-static RowShape row_shape(const RowGrid& g, int64_t D, int64_t T, int dtype) {
+static RowShape row_shape(const RowGrid& g, int64_t D, int64_t T, int dtype, bool backward) {
   const bool vec = g.vec;
   RowShape s{!vec ? kSingle : g.shifted() || D % g.ve != 0 ? kShifted : kAligned, false, false, 0, 0};
   const int ve = vec ? g.ve : 1;
@@ -741,7 +757,7 @@ static RowShape row_shape(const RowGrid& g, int64_t D, int64_t T, int dtype) {
     s.vpt = vec ? (nvec <= 32 ? 1 : 2) : 16;
     return s;
   }
-  s.vpt = T <= 2 * kNumSMs ? (vec ? 1 : 4) : (vec ? 4 : 16);
+  s.vpt = T <= 2 * kNumSMs ? (vec ? 1 : 4) : (vec ? (backward && dtype != FMOE_F32 && nvec <= 256 ? 2 : 4) : 16);
   while (s.vpt <= most && (nvec + s.vpt - 1) / s.vpt > row_threads(s.vpt * ve)) s.vpt *= vec ? 2 : 4;
   s.loop = s.vpt > most;
   s.threads = static_cast<int>(((nvec + s.vpt - 1) / s.vpt + 31) / 32 * 32);
@@ -784,9 +800,10 @@ static int launch_rows(const RowArgs& a, const RowShape& s, cudaStream_t st) {
 
 constexpr int kBwdWarps = 8;  // rows per CTA where a warp takes a row
 
-// Shared memory of rms_bwd_kernel: the weight and the next row's slots; a warp's rows only add up their dw in it.
+// Shared memory of rms_bwd_kernel: the weight (where a warp takes a row the sum of the warps' dw) and the next row's slots.
 static int bwd_smem(const RowShape& s, int64_t D, int ve) {
-  return s.warp ? 4 * static_cast<int>(D) : s.threads * s.vpt * (s.cut == kSingle ? 4 : 4 * ve + 3 * 16);
+  if (s.warp) return 4 * static_cast<int>((D + 3) / 4 * 4) + (s.cut == kSingle ? 0 : kBwdWarps * 3 * s.vpt * 32 * 16);
+  return s.threads * s.vpt * (s.cut == kSingle ? 4 : 4 * ve + 3 * 16);
 }
 
 template <int DT>
@@ -797,7 +814,7 @@ static int launch_bwd(const RowBwdArgs& a, const RowShape& s, int grid, cudaStre
   cudaError_t err = cudaSuccess;
 #define FMOE_ROWS(CUT, VPT, WARP)                                                                                \
   do {                                                                                                           \
-    if (smem > 48 * 1024)                                                                                        \
+    if (smem > 40 * 1024) /* 48 KB is the limit for this and the static part together */                         \
       err = cudaFuncSetAttribute(rms_bwd_kernel<DT, CUT, VPT, WARP>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
                                  smem);                                                                          \
     if (err == cudaSuccess) rms_bwd_kernel<DT, CUT, VPT, WARP><<<grid, block, smem, st>>>(a);                     \
@@ -810,14 +827,14 @@ static int launch_bwd(const RowBwdArgs& a, const RowShape& s, int grid, cudaStre
 }
 
 // CTAs of the backward pass, and so shares of dw: as many as the SMs hold at a time (128 registers a
-// thread), in a multiple of eight (see rms_bwd_kernel).
-static int bwd_grid(int64_t T, int threads, bool warp) {
-  const int per_sm = warp ? 4 : threads >= 512 ? 1 : threads <= 64 ? 8 : 512 / threads;
+// thread where a CTA takes a row), in a multiple of eight (see rms_bwd_kernel).
+static int bwd_grid(int64_t T, int threads, bool warp, int columns) {
+  const int per_sm = warp ? warp_ctas(columns) : threads >= 512 ? 1 : threads <= 64 ? 8 : 512 / threads;
   const int64_t rows = warp ? (T + kBwdWarps - 1) / kBwdWarps : T, most = per_sm * kNumSMs / 8 * 8;
   return static_cast<int>(rows < most ? rows : most);
 }
 // The size query knows neither the type nor the alignment: it answers for the fewest threads a row may get.
-static int bwd_grid_most(int64_t T, int64_t D) { return bwd_grid(T, static_cast<int>(D / 32 < 512 ? D / 32 : 512), false); }
+static int bwd_grid_most(int64_t T, int64_t D) { return bwd_grid(T, static_cast<int>(D / 32 < 512 ? D / 32 : 512), false, 0); }
 
 }  // namespace fmoe
 
@@ -848,7 +865,7 @@ extern "C" int fmoe_rms_norm(const void* x, int64_t x_stride, const void* residu
   g.weight(w);
   const RowArgs a{x, residual, w, y, sum, rstd, q, q_scale, T, D, x_stride, r_stride, q_stride, eps, 1.0 / static_cast<double>(D), w_dtype == FMOE_F32,
                   g.shift0, g.shift_step};
-  const RowShape s = row_shape(g, D, T, dtype);
+  const RowShape s = row_shape(g, D, T, dtype, false);
   int rc = FMOE_OK;
   FMOE_DISPATCH_DTYPE(dtype, DT, rc = (launch_rows<DT, true>(a, s, static_cast<cudaStream_t>(stream))));
   return rc;
@@ -868,7 +885,7 @@ extern "C" int fmoe_quantize_rows(const void* x, int64_t x_stride, int8_t* q, in
   g.add(x, x_stride, T);
   const RowArgs a{x, nullptr, nullptr, nullptr, nullptr, nullptr, q, q_scale, T, D, x_stride, 0, q_stride, 0.0, 0.0, 0,
                   g.shift0, g.shift_step};
-  const RowShape s = row_shape(g, D, T, dtype);
+  const RowShape s = row_shape(g, D, T, dtype, false);
   int rc = FMOE_OK;
   FMOE_DISPATCH_DTYPE(dtype, DT, rc = (launch_rows<DT, false>(a, s, static_cast<cudaStream_t>(stream))));
   return rc;
@@ -922,9 +939,9 @@ extern "C" int fmoe_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* 
   g.add(dsum, ds_stride, T);
   g.add(dx, D, T);
   g.weight(w);
-  RowShape s = row_shape(g, D, T, dtype);
+  RowShape s = row_shape(g, D, T, dtype, true);
   if (bwd_smem(s, D, g.ve) > 220 * 1024) s.loop = true;  // fp32 rows of more than 14000 columns
-  const int grid = s.loop ? bwd_grid_most(T, D) : bwd_grid(T, s.threads, s.warp);
+  const int grid = s.loop ? bwd_grid_most(T, D) : bwd_grid(T, s.threads, s.warp, s.vpt * (g.vec ? g.ve : 1));
   const RowBwdArgs a{dy, dsum, sum, rstd, w, dx, dw ? static_cast<float*>(scratch) : nullptr, T, D,
                      dy_stride, ds_stride, s_stride, 1.f / static_cast<float>(D), w_dtype == FMOE_F32, g.shift0, g.shift_step};
   int rc = FMOE_OK;

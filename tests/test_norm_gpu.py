@@ -14,7 +14,8 @@ DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 # one token and many; a warp's row and a block's; 16-byte vectors and single elements; widths around the
 # block shapes' borders, and rows too wide for registers
 SHAPES = [(1, 1), (1, 7168), (3, 64), (5, 63), (300, 257), (9, 1024), (2, 1032), (700, 2056), (7, 4099), (310, 4104),
-          (3, 8193), (2, 16384), (299, 16384), (2, 20001), (3, 33000)]  # fmt: skip
+          (3, 8193), (2, 16384), (299, 16384), (2, 20001), (3, 33000),
+          (400, 3001), (400, 814), (400, 600), (1300, 1000), (1300, 300)]  # fmt: skip
 
 
 def _inputs(T, D, dtype, wdtype=None, seed=0):
@@ -69,6 +70,19 @@ def _check_backward(gx, gw, s, w, dy, ds):
     term = dy.double() * xh
     ref = term.sum(0)
     assert_within(gw, ref, (T + 8) * U * term.abs().sum(0) + half(gw.dtype) * ref.abs() + smallest(gw.dtype), "dw")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_width_has_a_shape_that_launches(dtype):
+    """Block shapes and shared memory go by the width: a step of 61 columns passes through all of them."""
+    for T in (2, 300):
+        for D in range(61, 9000, 61):
+            x, r, dy, ds, w = _inputs(T, D, dtype)
+            x.requires_grad_(True)
+            w.requires_grad_(True)
+            y, s = norm.add_rms_norm(x, r, w, EPS)
+            gx, gw = torch.autograd.grad((y, s), (x, w), (dy, ds))
+    _check_backward(gx, gw, s.detach(), w.detach(), dy, ds)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
