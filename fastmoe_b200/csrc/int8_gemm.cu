@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(kFewThreads) int8_few_rows_kernel(const FewArg
     int lo = 0, hi = a.E;  // last e with chunk_prefix[e] * n_blocks <= item
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (chunk_prefix[mid] * f.n_blocks <= item) lo = mid; else hi = mid;
+      if (static_cast<int64_t>(chunk_prefix[mid]) * f.n_blocks <= item) lo = mid; else hi = mid;
     }
     const int chunks = chunk_prefix[lo + 1] - chunk_prefix[lo];
     const int local = item - chunk_prefix[lo] * f.n_blocks;
@@ -792,6 +792,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t tmem_base = *tmem_base_slot;
   const int items = chunk_prefix[a.E] * f.n_blocks;
   const int first = static_cast<int>(blockIdx.x) / f.splits, stride = static_cast<int>(gridDim.x) / f.splits;
+  // one item per cluster: there are enough of them unless experts claim the same rows
+  if (f.splits > 1 && items > stride && blockIdx.x == 0 && threadIdx.x == 0 && a.status != nullptr)
+    atomicOr(a.status, FMOE_STATUS_BAD_EXPERT);
 
   struct Item {
     int expert, nb, rows;
@@ -801,7 +804,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     int lo = 0, hi = a.E;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (chunk_prefix[mid] * f.n_blocks <= item) lo = mid; else hi = mid;
+      if (static_cast<int64_t>(chunk_prefix[mid]) * f.n_blocks <= item) lo = mid; else hi = mid;
     }
     const int chunks = chunk_prefix[lo + 1] - chunk_prefix[lo];
     const int local = item - chunk_prefix[lo] * f.n_blocks;

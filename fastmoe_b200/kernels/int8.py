@@ -198,7 +198,7 @@ def grouped_int8_gemm(a: Int8Rows, w: Int8Weight, offsets, counts, activation: i
     """Per expert e, over its rows [offsets[e], offsets[e] + counts[e]) (int64 [E] on the device): rows of
     a [R, K] times w[e] [N, K] transposed, both in 8 bits, then the activation (`experts.ACT_NONE`,
     `ACT_SWIGLU`: the first N/2 channels are the gate, or `ACT_GELU`), rounded once to `out_dtype`: [R, N], or
-    [R, N/2] for SwiGLU. Rows that belong to no expert read zero; `covers_all_rows=True` promises that
+    [R, N/2] for SwiGLU. No two experts may have a row in common. Rows that belong to no expert read zero; `covers_all_rows=True` promises that
     there are none, which saves the zero-fill."""
     _check_operands(a, w, 3, out_dtype)
     E, N = w.q.shape[:2]

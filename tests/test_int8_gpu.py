@@ -147,6 +147,40 @@ def test_a_range_past_the_rows_is_cut_off(R):
     _check(out, h, "none", torch.float32)
 
 
+def test_values_past_32_bits():
+    """More than 2^31 values in the rows, in the result and in the experts' weights."""
+    tail = 5
+    for R, K, N in (((1 << 31) // 8208 + 300, 8208, 8), ((1 << 31) // 8208 + 300, 16, 8208)):
+        a, w = _case(tail, K, N)
+        q = torch.zeros(R, K, dtype=torch.int8, device=DEV)
+        scale = torch.ones(R, device=DEV)
+        q[-tail:], scale[-tail:] = a.q, a.scale
+        out = int8.int8_linear(Int8Rows(q, scale), w)
+        assert not out[:-tail].any()
+        _check(out[-tail:], _product64(a, w.q, w.scale), "none", torch.bfloat16)
+    del q, out
+    E, K, N = 70, 8192, 4096
+    a, w = _case(tail, K, 1, N)
+    wq = torch.zeros(E, N, K, dtype=torch.int8, device=DEV)
+    ws = torch.ones(E, N, device=DEV)
+    wq[-1], ws[-1] = w.q[0], w.scale[0]
+    cnt = torch.zeros(E, dtype=torch.int64, device=DEV)
+    cnt[-1] = tail
+    out = int8.grouped_int8_gemm(a, Int8Weight(wq, ws), torch.zeros_like(cnt), cnt)
+    _check(out, _product64(a, w.q[0], w.scale[0]), "none", torch.bfloat16)
+
+
+def test_experts_that_claim_the_same_rows(kernel):
+    """Where this leaves rows without their product (the split-K kernel's clusters are counted by the rows)
+    the status word says so; nothing outside is touched."""
+    a, w = _case(32, 512, 4, 96)
+    off, cnt = torch.zeros(4, dtype=torch.int64, device=DEV), torch.full((4,), 32, dtype=torch.int64, device=DEV)
+    ops.read_status()
+    int8.grouped_int8_gemm(a, w, off, cnt)
+    torch.cuda.synchronize()
+    assert ops.read_status() == (_lib.STATUS_BAD_EXPERT if kernel == "split K" else 0)
+
+
 def test_operands_off_the_16_byte_grid_and_with_strides():
     g = _gen(3)
     base = torch.randint(-127, 128, (3, 41, 150), generator=g, device=DEV, dtype=torch.int8)
