@@ -14,6 +14,7 @@ unpacks as NaN.
 
 from __future__ import annotations
 
+import math
 from typing import NamedTuple
 
 import torch
@@ -59,6 +60,8 @@ def _check_packed(p: PackedActivation):
         raise ValueError("a packed activation's scales must be laid out as pack_activation returns them")
     if p.scale.device != p.q.device or p.dtype not in _DTYPES:
         raise ValueError("a packed activation's parts must live on one device and stand for a supported type")
+    if len(p.shape) < 1 or p.shape[-1] != D or math.prod(p.shape[:-1]) != T:
+        raise ValueError(f"a packed activation of shape {tuple(p.shape)} does not have [{T}, {D}] values")
     return T, D
 
 

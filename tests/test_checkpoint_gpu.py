@@ -98,6 +98,20 @@ def test_groups_of_zeros_and_of_infinities():
     assert torch.isfinite(back[1, :128]).all() and torch.isfinite(back[3]).all()
 
 
+def test_values_past_32_bits():
+    """More than 2^31 values: the last rows come out as they do alone."""
+    D, tail = 8200, 5
+    T = (1 << 31) // D + 300
+    x = torch.zeros(T, D, dtype=torch.bfloat16, device=DEV)
+    x[-tail:] = _x(tail, D, torch.bfloat16)
+    p, few = checkpoint.pack_activation(x), checkpoint.pack_activation(x[-tail:])
+    assert torch.equal(p.q[-tail:], few.q) and torch.equal(p.scale[-tail:], few.scale)
+    assert torch.equal(checkpoint.unpack_activation(p)[-tail:], checkpoint.unpack_activation(few))
+    for derivative, cols in ((checkpoint.packed_swiglu_backward, D // 2), (checkpoint.packed_gelu_backward, D)):
+        for got, want in zip(derivative(p, x[:, :cols]), derivative(few, x[-tail:, :cols])):
+            assert bool(want.any()) and torch.equal(got[-tail:], want)
+
+
 def test_no_rows_and_refusals():
     p = checkpoint.pack_activation(torch.empty(0, 64, device=DEV))
     assert checkpoint.unpack_activation(p).shape == (0, 64)
@@ -114,6 +128,11 @@ def test_no_rows_and_refusals():
         checkpoint.unpack_activation(p._replace(q=p.q.contiguous()))
     with pytest.raises(ValueError, match="laid out"):
         checkpoint.unpack_activation(p._replace(scale=p.scale[:2]))
+    for shape in ((2, 65), (4, 64), (2, 2, 66), ()):
+        with pytest.raises(ValueError, match="does not have"):
+            checkpoint.unpack_activation(p._replace(shape=torch.Size(shape)))
+        with pytest.raises(ValueError, match="does not have"):
+            checkpoint.packed_gelu_backward(p._replace(shape=torch.Size(shape)), x[: shape[0] if shape else 4])
     with pytest.raises(ValueError, match="float32/bfloat16/float16"):
         checkpoint.pack_activation(x.double())
     with pytest.raises(RuntimeError, match="no CPU path"):
