@@ -22,7 +22,7 @@ import torch
 
 from .. import _lib
 from . import ops
-from .int8 import Int8Rows, _operand, _padded
+from .int8 import Int8Rows, _check_rows, _operand, _padded
 from .ops import _DTYPES, _require_cuda, _status_word, _stream_ptr
 
 
@@ -162,6 +162,7 @@ def permute_rows(x: torch.Tensor, slot_of: torch.Tensor, K: int) -> torch.Tensor
 
 def permute_int8_rows(rows: Int8Rows, ix: RoutingIndex, K: int) -> Int8Rows:
     """The dispatch permute for rows in 8 bits: a token's bytes and scale at every sorted slot of it."""
+    _check_rows(rows.q, rows.scale)
     q = _operand(rows.q)
     T, D = q.shape
     if D % 16:  # the rows travel with their padding, as 16-bit words

@@ -299,4 +299,10 @@ def test_refusals():
     lin = Int8Linear(torch.nn.Linear(16, 8, bias=False).to(DEV)).to(BF16)
     with pytest.raises(ValueError, match="scale must be float32"):
         lin(torch.randn(2, 16, device=DEV, dtype=BF16))
+    ix = routing.build_index(torch.zeros(4, 1, dtype=torch.int64, device=DEV), torch.ones(4, 1, device=DEV), 2)
+    rows = int8.quantize_rows(torch.randn(4, 32, device=DEV))
+    with pytest.raises(ValueError, match="q must be int8"):
+        routing.permute_int8_rows(rows._replace(q=rows.q.float()), ix, 1)
+    with pytest.raises(ValueError, match="scale must be float32"):
+        routing.permute_int8_rows(rows._replace(scale=rows.scale[:3]), ix, 1)
     assert RMSNorm(8).weight.shape == (8,)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from eight_bit import U, assert_quantised, assert_within, half, quantise, smallest
-from fastmoe_b200.kernels import norm
+from fastmoe_b200.kernels import int8, norm
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -134,6 +134,27 @@ def test_a_row_does_not_depend_on_its_batch(T):
         one = norm.rms_norm_int8(x[-1:], w, EPS, residual=r[-1:], with_y=True)
         assert torch.equal(out.rows.q[-1:], one.rows.q) and torch.equal(out.rows.scale[-1:], one.rows.scale)
         assert torch.equal(out.y[-1:], one.y)
+
+
+@pytest.mark.parametrize("D", [8200, 8203, 200])
+def test_values_past_32_bits(D):
+    """More than 2^31 values, in each form of the kernels: the last rows come out as they do alone."""
+    T, tail = (1 << 31) // D + 300, 5
+    x = torch.zeros(T, D, dtype=torch.bfloat16, device=DEV)
+    x[-tail:], r, dy, ds, w = _inputs(tail, D, torch.bfloat16)
+    grads = torch.zeros_like(x)
+    grads[-tail:] = dy
+    few = x[-tail:].clone()
+    xg, wg = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    gx, gw = torch.autograd.grad(norm.rms_norm(xg, wg, EPS), (xg, wg), grads)
+    _check_backward(gx[-tail:], gw, few, w, dy, None)  # rows of zeros add nothing to dw
+    assert not gx[:-tail].any()
+    del gx, grads, xg
+    rows, alone = int8.quantize_rows(x), int8.quantize_rows(few)
+    assert torch.equal(rows.q[-tail:], alone.q) and torch.equal(rows.scale[-tail:], alone.scale)
+    assert torch.equal(int8.dequantize_rows(rows)[-tail:], int8.dequantize_rows(alone))
+    out, alone = norm.rms_norm_int8(x, w, EPS, with_y=True), norm.rms_norm_int8(few, w, EPS, with_y=True)
+    assert torch.equal(out.rows.q[-tail:], alone.rows.q) and torch.equal(out.y[-tail:], alone.y)
 
 
 @pytest.mark.parametrize("D", [200, 204, 2051])
