@@ -872,6 +872,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int64_t col = static_cast<int64_t>(t.nb) * out_cols + (line & (out_cols - 1));
       const bool up = swiglu && line >= 64;
       const float sw = col < a.cols ? a.w_scale[static_cast<int64_t>(t.expert) * a.N + (up ? a.cols : 0) + col] : 0.f;
+      // lane j has the scales of tokens j, j + 32, ..: here, not where they are used, 0.7 us away from memory each
+      float sa[(NB + 31) / 32];
+#pragma unroll
+      for (int j = 0; j < (NB + 31) / 32; ++j) sa[j] = 32 * j + lane < t.rows ? a.a_scale[t.row0 + 32 * j + lane] : 0.f;
       if (epilogue_any(!mbar_wait(&tmem_full[acc], (it >> 1) & 1, abort_flag, a.spin_limit))) goto timed_out;
       tcgen05_fence_after();
       const uint32_t taddr = tmem_base + acc * NB + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -885,10 +889,13 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int i = 0; i < 16; ++i) part[(c0 + i) * kTnRows + line] = static_cast<int>(r[i]);
           continue;
         }
-        const float mine = c0 + (lane & 15) < t.rows ? a.a_scale[t.row0 + c0 + (lane & 15)] : 0.f;
+        float mine = sa[0];
+#pragma unroll
+        for (int j = 1; j < (NB + 31) / 32; ++j) mine = c0 >= 32 * j ? sa[j] : mine;
         float y[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = static_cast<float>(static_cast<int>(r[i])) * __shfl_sync(0xffffffffu, mine, i) * sw;
+        for (int i = 0; i < 16; ++i)
+          y[i] = static_cast<float>(static_cast<int>(r[i])) * __shfl_sync(0xffffffffu, mine, (c0 & 16) + i) * sw;
         if (swiglu) {
           if (up) {
 #pragma unroll
@@ -945,6 +952,14 @@ done:
       const int64_t col = static_cast<int64_t>(t.nb) * out_cols + c;
       if (col >= a.cols) continue;
       const uint32_t at = base + 4 * (token * kTnRows + c);
+      const float sa = a.a_scale[t.row0 + token];  // the scales on their way before the sums
+      float sg[4], su[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t n = col + j < a.cols ? col + j : col;
+        sg[j] = scales[n];
+        su[j] = swiglu ? scales[a.cols + n] : 0.f;
+      }
       int4 sum = make_int4(0, 0, 0, 0), up = sum;
 #pragma unroll 8
       for (int r = 0; r < f.splits; ++r) {
@@ -958,14 +973,12 @@ done:
           up.x += v.x, up.y += v.y, up.z += v.z, up.w += v.w;
         }
       }
-      const float sa = a.a_scale[t.row0 + token];
       const int sums[4] = {sum.x, sum.y, sum.z, sum.w}, ups[4] = {up.x, up.y, up.z, up.w};
       float y[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int64_t n = col + j < a.cols ? col + j : col;
-        y[j] = static_cast<float>(sums[j]) * sa * scales[n];
-        if (swiglu) y[j] = y[j] * sigmoid(y[j]) * (static_cast<float>(ups[j]) * sa * scales[a.cols + n]);
+        y[j] = static_cast<float>(sums[j]) * sa * sg[j];
+        if (swiglu) y[j] = y[j] * sigmoid(y[j]) * (static_cast<float>(ups[j]) * sa * su[j]);
         else if (a.act == FMOE_ACT_GELU) y[j] = gelu(y[j]);
       }
       store4(a.C, (t.row0 + token) * a.cols + col, a.out_dtype, y, static_cast<int>(a.cols - col < 4 ? a.cols - col : 4),
