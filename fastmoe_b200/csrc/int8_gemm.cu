@@ -467,7 +467,6 @@ done:
 // tile shape that counts.
 constexpr int kFewThreads = 256, kFewWarps = 8, kFewRows = 32;  // weight rows per CTA
 constexpr int kFewStep = 128;                                  // bytes of K per warp and step
-constexpr int64_t kFewBytes = 16 << 20, kFewTokens = 256;  // weight bytes times passes, see fmoe_int8_gemm
 constexpr int kFewPad = 4;  // columns of padding in the reduction buffer: fragment stores without bank conflicts
 
 struct FewArgs {
@@ -672,14 +671,11 @@ struct TnArgs {
   int splits;    // CTAs per cluster, each with its share of K; 1: a persistent grid
 };
 
-// Four integers at `saddr` of CTA `rank`'s shared memory. Not volatile: the loads of one output go out
-// together. (A volatile load per CTA and output, one after the other, cost 20 us at 128 tokens.)
-__device__ __forceinline__ int4 ld_cluster4(uint32_t saddr, uint32_t rank) {
+// One integer into CTA `rank`'s shared memory, at the place that `saddr` is in this CTA's.
+__device__ __forceinline__ void st_cluster(uint32_t saddr, uint32_t rank, uint32_t v) {
   uint32_t remote;
-  int4 v;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(saddr), "r"(rank));
-  asm("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(remote) : "memory");
-  return v;
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
 }
 // Barrier of the four epilogue warps that also tells whether one of them gave up: a warp must not wait
 // here for one that has left.
@@ -715,6 +711,15 @@ __device__ __forceinline__ void store4(void* C, int64_t i, int dt, const float* 
   }
 }
 
+// The first n of 16 outputs of one column.
+template <int DT>
+__device__ __forceinline__ void store_column(void* C, int64_t at, int64_t stride, const float* y, int n) {
+  typename Elem<DT>::type* p = static_cast<typename Elem<DT>::type*>(C) + at;
+#pragma unroll
+  for (int i = 0; i < 16; ++i, p += stride)
+    if (i < n) *p = from_float<DT>(y[i]);
+}
+
 template <int NB>
 __global__ void __launch_bounds__(kThreads, 2)
     int8_tn_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_w, const TnArgs f) {
@@ -732,7 +737,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint64_t* drain = reinterpret_cast<uint64_t*>(abort_flag + 1);
   float* exchange = reinterpret_cast<float*>(smem + kS * kStage + 256);
   int* chunk_prefix = reinterpret_cast<int*>(exchange + kTnExchange);  // [E + 1]
-  int* part = reinterpret_cast<int*>(smem);                            // [NB][128], after the pipeline has drained
+  // partial sums from each CTA of the cluster for this CTA's tokens, after the pipelines have drained
+  int* part = reinterpret_cast<int*>(smem);                            // [splits][NB / splits][128]
 
   const Args& a = f.g;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -877,6 +883,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int j = 0; j < (NB + 31) / 32; ++j) sa[j] = 32 * j + lane < t.rows ? a.a_scale[t.row0 + 32 * j + lane] : 0.f;
       if (epilogue_any(!mbar_wait(&tmem_full[acc], (it >> 1) & 1, abort_flag, a.spin_limit))) goto timed_out;
+      if (f.splits > 1) break;  // one item per cluster: its sums meet below
       tcgen05_fence_after();
       const uint32_t taddr = tmem_base + acc * NB + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
@@ -884,11 +891,6 @@ __global__ void __launch_bounds__(kThreads, 2)
         uint32_t r[16];
         tmem_ld16(taddr + c0, r);
         tmem_ld_wait();
-        if (f.splits > 1) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) part[(c0 + i) * kTnRows + line] = static_cast<int>(r[i]);
-          continue;
-        }
         float mine = sa[0];
 #pragma unroll
         for (int j = 1; j < (NB + 31) / 32; ++j) mine = c0 >= 32 * j ? sa[j] : mine;
@@ -912,9 +914,11 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int i = 0; i < 16; ++i) y[i] = gelu(y[i]);
         }
         if (!up && col < a.cols) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (c0 + i < t.rows) store_scalar_from_float(a.C, (t.row0 + c0 + i) * a.cols + col, a.out_dtype, y[i]);
+          const int64_t at = (t.row0 + c0) * a.cols + col;
+          const int n = t.rows - c0;
+          if (a.out_dtype == FMOE_F32) store_column<FMOE_F32>(a.C, at, a.cols, y, n);
+          else if (a.out_dtype == FMOE_BF16) store_column<FMOE_BF16>(a.C, at, a.cols, y, n);
+          else store_column<FMOE_F16>(a.C, at, a.cols, y, n);
         }
       }
       tcgen05_fence_before();
@@ -932,61 +936,77 @@ done:
   drain_on_exit(warp, lane, fills, mma_issued, full, drain, abort_flag, kS, a.spin_limit);
   tcgen05_fence_before();
   __syncthreads();
+  // A cluster's CTAs each finish every splits-th token: they send each other their partial sums, and each adds
+  // up what it got from its own shared memory. (Fetching the others' sums instead, a round trip for every
+  // one, took 20.0 us where this takes 18.4 for 128 rows of 7168 x 7168 in four parts.)
+  // All threads of all its CTAs come here, also after a wait gave up.
+  const int quads = out_cols / 4, c = static_cast<int>(threadIdx.x) % quads * 4;  // kThreads is a multiple of quads
+  Item t{0, 0, 0, 0};
+  int64_t col = 0;
+  float sg[4], su[4];
+  if (f.splits > 1) {
+    if (first < items) {
+      t = find(first);
+      col = static_cast<int64_t>(t.nb) * out_cols + c;
+      const float* scales = a.w_scale + static_cast<int64_t>(t.expert) * a.N;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sg[j] = col + j < a.cols ? scales[col + j] : 0.f;
+        su[j] = swiglu && col + j < a.cols ? scales[a.cols + col + j] : 0.f;
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();  // every CTA's pipeline has drained
+    tcgen05_fence_after();
+    if (warp >= 2) {
+      const int quarter = warp & 3, shift = __ffs(f.splits) - 1;
+      const uint32_t mine = smem_u32(part + split * (NB * kTnRows >> shift) + quarter * 32 + lane);
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll 1
+      for (int c0 = 0; c0 < t.rows; c0 += 16) {
+        uint32_t r[16];
+        tmem_ld16(taddr + c0, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (c0 + i < t.rows) st_cluster(mine + 4 * kTnRows * ((c0 + i) >> shift), i & (f.splits - 1), r[i]);
+      }
+    }
+    tcgen05_fence_before();
+    __syncwarp();
+    cluster_sync_all();
+  }
   if (warp == 1) {
     __syncwarp();
     tcgen05_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "n"(kTmemCols) : "memory");
   }
-  if (f.splits == 1) return;
-  // One item per cluster: every CTA adds up its share of the outputs over the cluster's partial sums.
-  // All threads of all its CTAs come here, also after a wait gave up.
-  __syncwarp();
-  cluster_sync_all();
-  if (first < items) {
-    const Item t = find(first);
-    const uint32_t base = smem_u32(part);
-    const float* scales = a.w_scale + static_cast<int64_t>(t.expert) * a.N;
-    // four neighbouring columns of a token at a time
-    for (int i = split * kThreads + threadIdx.x; i < t.rows * (out_cols / 4); i += f.splits * kThreads) {
-      const int token = i / (out_cols / 4), c = (i - token * (out_cols / 4)) * 4;
-      const int64_t col = static_cast<int64_t>(t.nb) * out_cols + c;
-      if (col >= a.cols) continue;
-      const uint32_t at = base + 4 * (token * kTnRows + c);
-      const float sa = a.a_scale[t.row0 + token];  // the scales on their way before the sums
-      float sg[4], su[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t n = col + j < a.cols ? col + j : col;
-        sg[j] = scales[n];
-        su[j] = swiglu ? scales[a.cols + n] : 0.f;
-      }
-      int4 sum = make_int4(0, 0, 0, 0), up = sum;
-#pragma unroll 8
-      for (int r = 0; r < f.splits; ++r) {
-        const int4 v = ld_cluster4(at, r);
-        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-      }
+  if (f.splits == 1 || col >= a.cols) return;
+  // four neighbouring columns of a token to a thread
+  for (int i = static_cast<int>(threadIdx.x) / quads; i * f.splits + split < t.rows; i += kThreads / quads) {
+    const int64_t row = t.row0 + i * f.splits + split;
+    const float sa = a.a_scale[row];
+    const int* from = part + i * kTnRows + c;
+    int4 sum = make_int4(0, 0, 0, 0), up = sum;
+    for (int r = 0; r < f.splits; ++r, from += NB * kTnRows / f.splits) {
+      const int4 v = *reinterpret_cast<const int4*>(from);
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
       if (swiglu) {
-#pragma unroll 8
-        for (int r = 0; r < f.splits; ++r) {
-          const int4 v = ld_cluster4(at + 4 * 64, r);
-          up.x += v.x, up.y += v.y, up.z += v.z, up.w += v.w;
-        }
+        const int4 w = *reinterpret_cast<const int4*>(from + 64);
+        up.x += w.x, up.y += w.y, up.z += w.z, up.w += w.w;
       }
-      const int sums[4] = {sum.x, sum.y, sum.z, sum.w}, ups[4] = {up.x, up.y, up.z, up.w};
-      float y[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        y[j] = static_cast<float>(sums[j]) * sa * sg[j];
-        if (swiglu) y[j] = y[j] * sigmoid(y[j]) * (static_cast<float>(ups[j]) * sa * su[j]);
-        else if (a.act == FMOE_ACT_GELU) y[j] = gelu(y[j]);
-      }
-      store4(a.C, (t.row0 + token) * a.cols + col, a.out_dtype, y, static_cast<int>(a.cols - col < 4 ? a.cols - col : 4),
-             a.cols % 4 == 0 && a.vec_ok != 0);
     }
+    const int sums[4] = {sum.x, sum.y, sum.z, sum.w}, ups[4] = {up.x, up.y, up.z, up.w};
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      y[j] = static_cast<float>(sums[j]) * sa * sg[j];
+      if (swiglu) y[j] = y[j] * sigmoid(y[j]) * (static_cast<float>(ups[j]) * sa * su[j]);
+      else if (a.act == FMOE_ACT_GELU) y[j] = gelu(y[j]);
+    }
+    store4(a.C, row * a.cols + col, a.out_dtype, y, static_cast<int>(a.cols - col < 4 ? a.cols - col : 4),
+           a.cols % 4 == 0 && a.vec_ok != 0);
   }
-  __syncwarp();
-  cluster_sync_all();  // no CTA leaves while another reads its sums
 }
 
 // int8 tensor [depth, rows, cols] with the given strides in bytes (depth 1: [rows, cols]), box =
@@ -1077,6 +1097,45 @@ static int launch_tiles(const CUtensorMap& map_a, const CUtensorMap& map_w, cons
   return check_launch("int8_gemm_kernel");
 }
 
+// Kernel 0 (tiles), 1 (few rows), 2 (weight rows as M) or 3 (pairs) for E experts of which `reached` can have rows,
+// `mean` rows each. The first two by an estimate of their times in us, fitted to (few / 2 / tiles): 512 x
+// 4096, 16 rows 3.2 / 4.2 / 6.9, 64 rows 7.6 / 5.1 / 7.2; 2048 x 7168, 8 rows 5.9 / 8.2 / 12.9, 24 rows 10.5 /
+// 8.5 / 13.2; 7168 x 7168, 8 rows 13.9 / 15.4 / 33, 16 rows 20.8 / 15.5 / 33; 8192 x 1024, 1 row 7.6 / 6.8 / 26;
+// 1008 x 515, 256 rows 6.0 / 8.3 / 13.8: few rows pays for every 8 tokens by 32 weight rows, kernel 2 for the weights
+// once and for its start and end. The tiled kernel (2 / tiles / pairs) streams fewer bytes per product but
+// needs tiles for most SMs and starts 2 us later: 7168 x 7168, 256 rows 24.7 / 29.5 / 27.2, 512 rows 30.0 / 29.2 / 27.3;
+// 2048 x 7168, 1024 rows 19.7 / 20.4 / 20.4, 2048 rows 31.2 / 29.9 / 30.9; 64 experts of 7168 x 4096 with SwiGLU, 64 rows
+// each 294 / 293, 128 each 375 / 361. Pairs of CTAs gain on a long K where their tiles of 256 rows do not cost a round
+// more: 7168 x 21504, 256 rows 55.8 / 49.8, 384 rows 54.7 / 62.7, 512 rows 75 / 65; 8192 x 8192, 32768 rows for seconds on
+// end (at the power limit) 1680 / 1620; experts' rows come in ragged numbers, and pad them at a few hundred
+// (32 experts of 7168 x 4096, 256 rows each 263 / 292, 2048 rows for seconds on end 1490 / 1440).
+static int pick_kernel(const Args& g, int64_t K, int64_t reached, int64_t mean, int64_t few_items, int nb, int64_t tn_items) {
+  const double weights = static_cast<double>(reached) * static_cast<double>(g.N) * static_cast<double>(K);
+  const double rounds = few_items > kNumSMs ? static_cast<double>(few_items) / kNumSMs : 1.0;
+  const double few = 2.4 + fmax(rounds * (0.45 + 0.55 * static_cast<double>(K) / 1024), weights / 5e6);
+  const double tn = 4.2 + fmax(0.245 * (g.k_blocks < 12 ? g.k_blocks : 12) - 1.0, weights / 6e6) + nb / 64.0;
+  const bool long_k = K >= 4096;
+  if (mean <= 64 || tn_items <= (long_k || g.act == FMOE_ACT_SWIGLU ? 1 : 4) * kNumSMs) return few < tn ? 1 : 2;
+  if (!long_k) return 0;
+  if (g.E > 1) return mean < 1024 ? 0 : 3;
+  const int64_t tiles = (g.R + kBM - 1) / kBM * g.n_blocks, pairs = (g.R + 2 * kBM - 1) / (2 * kBM) * g.n_blocks;
+  return (pairs + kNumSMs / 2 - 1) / (kNumSMs / 2) <= (tiles + kNumSMs - 1) / kNumSMs ? 3 : 0;
+}
+
+// Parts of K for the CTAs of a cluster, for as long as there are CTAs to spare (two to an SM). A part saves its k
+// blocks (0.25 us each); the exchange costs 1.5 us, 2 to 4 in two parts, and more when the SMs are full.
+// Measured (1 / 2 / 4 / 8 parts, us; 128 rows): 1024 x 512 7.2 / 10.4 / 8.2 / 7.4, 2048 x 512 9.3 / 11.4 / 8.7 / 7.5, 2048 x
+// 2048 9.3 / 11.4 / 8.8 / 9.6, 7168 x 2048 24.6 / 19.4 / 13.3 / 12.3, 2048 x 7168 11.3 / 13.2 / 12.8, 4096 x 7168 17.4 / 17.0 /
+// 15.2; 256 rows: 4096 x 7168 17.6 / 19.2, 7168 x 7168 26.4 / 24.5.
+static int pick_splits(int64_t items, int k_blocks) {
+  for (int parts = 8; parts > 1 && k_blocks >= 12; parts /= 2) {
+    const int64_t ctas = items * parts;
+    const int least = parts == 2 ? 20 : ctas > kNumSMs ? 8 : 2 * ctas > kNumSMs ? 4 : 2;  // k blocks of a part
+    if (ctas <= 2 * kNumSMs && k_blocks / parts >= least) return parts;
+  }
+  return 1;
+}
+
 }  // namespace i8
 
 int g_int8_kernel = -1;  // fmoe_tune "int8_kernel": 0 tiles, 1 few rows, 2 split K, 3 pairs; -1 = by the sizes
@@ -1128,22 +1187,15 @@ extern "C" int fmoe_int8_gemm(const int8_t* a, int64_t a_stride, const float* a_
   g.status = status;
   FMOE_REQUIRE((R / i8::kBM + E) * g.n_blocks < (1ll << 31), FMOE_ERR_UNSUPPORTED, "fmoe_int8_gemm: too many tiles");
   // Which kernel: the host knows the rows and the experts, not how the rows are spread.
-  const int64_t mean = (R + E - 1) / E, touched = (R < E ? R : E) * N * K;
+  const int64_t reached = R < E ? R : E, mean = (R + E - 1) / E;
   const int64_t tokens = E == 1 ? R : 2 * mean;  // rows that an expert may well have
+  const int few_blocks = static_cast<int>(swiglu ? (cols + 15) / 16 : (N + i8::kFewRows - 1) / i8::kFewRows);
+  const int64_t few_items = (E == 1 ? (R + 7) / 8 : R / 8 + reached) * few_blocks;
+  const int tn_blocks = static_cast<int>(swiglu ? (cols + 63) / 64 : (N + i8::kTnRows - 1) / i8::kTnRows);
+  const int nb = tokens <= 16 ? 16 : tokens <= 32 ? 32 : tokens <= 64 ? 64 : 128;
+  const int64_t tn_items = (E == 1 ? (R + nb - 1) / nb : R / nb + reached) * tn_blocks;
   int which = g_int8_kernel;
-  if (which < 0) {
-    const int64_t tiles = ((R + i8::kBM - 1) / i8::kBM + (R < E ? R : E) - 1) * g.n_blocks;
-    // One pass over the weights for every eight rows of an expert costs the few-rows kernel 2 us per 16 MB
-    // after a start of 3 us; the split-K kernel starts at 5 to 6 us and the tiled one at 8 to 9 us. Measured
-    // (few / split K / tiled, us): 512 x 4096, 8 rows 3.4 / 5.8 / 8.8, 64 rows 7.9 / 9.1 / 9.2; 2048 x 7168, 8
-    // rows 6.6 / 8.9 / 16.6, 24 rows 11.3 / 9.5 / 17.0. A tile of the tiled kernel takes the same time for 1 row
-    // and for 128, so it needs tiles for most SMs: 7168 x 7168, 256 rows (56 tiles) - / 26 / 33, 512 rows
-    // (112) - / 35 / 32; 64 experts of 7168 x 4096, 32 rows each - / 282 / 292, 128 each - / 359 / 339. Pairs of CTAs: 8192 x 8192,
-    // 1024 rows 57 -> 52, 32768 rows for seconds on end (at the power limit) 1680 -> 1620; their 256-row tiles pad
-    // an expert of a few hundred rows more than that gains (32 experts of 7168 x 4096, 256 rows 263 -> 292, 1024
-    // rows 726 -> 725, 2048 rows for seconds on end 1490 -> 1440).
-    which = tokens <= i8::kFewTokens && (tokens + 7) / 8 * touched <= i8::kFewBytes ? 1 : mean <= 64 || tiles <= 56 ? 2 : mean < 1024 ? 0 : 3;
-  }
+  if (which < 0) which = i8::pick_kernel(g, K, reached, mean, few_items, nb, tn_items);
   if (which == 1) {
     i8::FewArgs f;
     f.A = a;
@@ -1152,33 +1204,29 @@ extern "C" int fmoe_int8_gemm(const int8_t* a, int64_t a_stride, const float* a_
     f.w_stride = w_stride;
     f.w_expert_stride = E == 1 ? 0 : w_expert_stride;
     f.K = K;
-    f.n_blocks = static_cast<int>(swiglu ? (cols + 15) / 16 : (N + i8::kFewRows - 1) / i8::kFewRows);
+    f.n_blocks = few_blocks;
     f.g = g;
-    const int64_t items = (R / 8 + (R < E ? R : E)) * f.n_blocks;
-    FMOE_REQUIRE(items < (1ll << 31), FMOE_ERR_UNSUPPORTED, "fmoe_int8_gemm: too many tiles");
+    FMOE_REQUIRE(few_items < (1ll << 31), FMOE_ERR_UNSUPPORTED, "fmoe_int8_gemm: too many tiles");
     int rc = FMOE_OK;
-    FMOE_DISPATCH_DTYPE(out_dtype, DT, rc = (i8::launch_few<DT, 1>(f, items, static_cast<cudaStream_t>(stream))));
+    FMOE_DISPATCH_DTYPE(out_dtype, DT, rc = (i8::launch_few<DT, 1>(f, few_items, static_cast<cudaStream_t>(stream))));
     return rc;
   }
   if (which == 2) {
     i8::TnArgs f;
     f.g = g;
-    f.n_blocks = static_cast<int>(swiglu ? (cols + 63) / 64 : (N + i8::kTnRows - 1) / i8::kTnRows);
-    const int nb = tokens <= 16 ? 16 : tokens <= 32 ? 32 : tokens <= 64 ? 64 : 128;
-    const int64_t items = (E == 1 ? (R + nb - 1) / nb : R / nb + (R < E ? R : E)) * f.n_blocks;
-    FMOE_REQUIRE(items < (1ll << 31) / 8, FMOE_ERR_UNSUPPORTED, "fmoe_int8_gemm: too many tiles");
-    f.splits = 1;
-    while (f.splits < 8 && items * f.splits * 2 <= 2 * kNumSMs && g.k_blocks / (f.splits * 2) >= 2) f.splits *= 2;
+    f.n_blocks = tn_blocks;
+    FMOE_REQUIRE(tn_items < (1ll << 31) / 8, FMOE_ERR_UNSUPPORTED, "fmoe_int8_gemm: too many tiles");
+    f.splits = i8::pick_splits(tn_items, g.k_blocks);
     CUtensorMap map_t, map_w;
     int rc = i8::make_map(&map_t, a, 1, R, K, a_stride, R * a_stride, nb, 2, "A");
     if (rc != 0) return rc;
     rc = i8::make_map(&map_w, w, E, N, K, w_stride, E == 1 ? N * w_stride : w_expert_stride, swiglu ? 64 : i8::kTnRows, 3, "W");
     if (rc != 0) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (nb == 16) return i8::launch_tn<16>(map_t, map_w, f, items, st);
-    if (nb == 32) return i8::launch_tn<32>(map_t, map_w, f, items, st);
-    if (nb == 64) return i8::launch_tn<64>(map_t, map_w, f, items, st);
-    return i8::launch_tn<128>(map_t, map_w, f, items, st);
+    if (nb == 16) return i8::launch_tn<16>(map_t, map_w, f, tn_items, st);
+    if (nb == 32) return i8::launch_tn<32>(map_t, map_w, f, tn_items, st);
+    if (nb == 64) return i8::launch_tn<64>(map_t, map_w, f, tn_items, st);
+    return i8::launch_tn<128>(map_t, map_w, f, tn_items, st);
   }
   CUtensorMap map_a, map_w;
   int rc = i8::make_map(&map_a, a, 1, R, K, a_stride, R * a_stride, i8::kBM, 2, "A");
