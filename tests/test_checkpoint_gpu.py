@@ -85,6 +85,31 @@ def test_strides_leading_dimensions_and_autograd_leaves():
     assert torch.equal(h, checkpoint.packed_gelu_backward(pt, one.contiguous())[1])
 
 
+@pytest.mark.parametrize("D", [512, 300])
+def test_on_a_side_stream_and_in_a_graph(D):
+    """Captured once, replayed on new values, beside eager calls on another stream."""
+    x, grad, side = _x(70, D, torch.bfloat16), _x(70, D // 2, torch.bfloat16, seed=3), torch.cuda.Stream()
+
+    def run():
+        p = checkpoint.pack_activation(x)
+        return (p.q, p.scale, checkpoint.unpack_activation(p), *checkpoint.packed_swiglu_backward(p, grad))
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        captured = run()
+    x.copy_(_x(70, D, torch.bfloat16, seed=9))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        with torch.cuda.stream(side):
+            graph.replay()
+        eager = run()
+    torch.cuda.synchronize()
+    for a, b in zip(captured, eager):
+        assert torch.equal(a, b)
+
+
 def test_groups_of_zeros_and_of_infinities():
     x = _x(4, 384, torch.float32)
     x[0, :128] = 0

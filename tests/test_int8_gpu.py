@@ -55,7 +55,9 @@ def _check(out, h, act, dtype):
 
 LINEAR = [(1, 1, 1), (1, 16, 8), (1, 7168, 515), (2, 15, 33), (3, 17, 64), (7, 127, 100), (8, 128, 256), (9, 129, 257),
           (16, 1000, 255), (17, 640, 130), (32, 96, 31), (33, 2048, 1024), (48, 7168, 300), (64, 512, 4100), (65, 200, 96),
-          (100, 1001, 513), (128, 128, 256), (129, 144, 20), (200, 4096, 7), (300, 320, 1999), (1000, 1024, 768)]  # fmt: skip
+          (100, 1001, 513), (128, 128, 256), (129, 144, 20), (200, 4096, 7), (300, 320, 1999), (1000, 1024, 768),
+          # K in 2, 4 and 8 parts with 128, 32 and 16 tokens to a tile, and in 4 with ragged ones
+          (256, 5200, 7168), (20, 4104, 7100), (16, 4111, 600), (130, 2304, 515)]  # fmt: skip
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
@@ -93,6 +95,7 @@ GROUPED = [
     ([128, 256, 127, 129], 130, 258),
     ([700, 33], 1000, 250),
     ([2100, 1, 2050], 192, 600),  # more row blocks than share their column blocks' weights
+    ([40], 4104, 7168), ([9, 0, 7], 2048, 384), ([31, 20, 0, 3], 3333, 259), ([100, 28], 2000, 512),  # a long K in parts
 ]
 
 
@@ -333,7 +336,8 @@ def test_norm_to_experts_together(act, ffn):
 def test_on_a_side_stream_and_in_graphs():
     """Two captured graphs of the same call, replayed on two streams at once, and an eager call between
     them: no memory is shared between calls."""
-    cases = [_case(5, 512, 300, seed=4), _case(300, 512, 300, seed=5), _case(2100, 256, 300, seed=6)]
+    cases = [_case(5, 512, 300, seed=4), _case(300, 512, 300, seed=5), _case(2100, 256, 300, seed=6),
+             _case(48, 7168, 300, seed=7), _case(130, 4096, 1000, seed=8)]  # fmt: skip
     streams, graphs, outs = [torch.cuda.Stream() for _ in cases], [], []
     for (a, w), s in zip(cases, streams):
         int8.int8_linear(a, w)
