@@ -305,7 +305,7 @@ def _launch(device: int, fn_name, n_kernels, *args):
     device made current for the launch where it is not. Small calls are bound by what happens on the
     host before the launch: the stream's raw handle saves 2 us against a torch.cuda.Stream."""
     global launch_count
-    if device != torch.cuda.current_device():
+    if device != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return _launch(device, fn_name, n_kernels, *args)
     stream = torch._C._cuda_getCurrentRawStream(device)
