@@ -448,23 +448,43 @@ class MoEFeedForward(nn.Module):
     def quantize_int8(self):
         """From now on `forward` runs the experts in 8-bit integers (kernels/int8.py), for inference: the
         weights are quantised here, once, with a scale per output channel. The router stays as it is.
-        The floating-point weights are kept; `dequantize()` returns to them. Single rank only."""
+        The floating-point weights are kept; `dequantize()` returns to them. Where they have been written or
+        replaced since (`load_state_dict`, an update in place), the next `forward` quantises them again. A
+        write that torch does not count (through `.data`), and a captured graph, need this call again: it
+        refreshes the 8-bit weights in place. Single rank only."""
         if self.world_size > 1 or getattr(self, "_fused_exchange", None) is not None:
             raise ValueError("experts in int8 run on a single rank: rows do not travel in 8 bits")
+        marks = self._weight_marks()
         if self.expert_type == "swiglu":
             w1, w2 = int8.quantize_weight(self.experts.w_gate_up), int8.quantize_weight(self.experts.w_down)
         else:
             w1 = int8.quantize_weight(torch.stack([expert[0].weight.detach() for expert in self.experts]))
             w2 = int8.quantize_weight(torch.stack([expert[2].weight.detach() for expert in self.experts]))
-        for name, w in (("w1", w1), ("w2", w2)):
-            self.register_buffer(f"{name}_q", w.q, persistent=False)
-            self.register_buffer(f"{name}_scale", w.scale, persistent=False)
+        for name, t in (("w1_q", w1.q), ("w1_scale", w1.scale), ("w2_q", w2.q), ("w2_scale", w2.scale)):
+            old = self._buffers.get(name)
+            if (old is None or old.shape != t.shape or old.dtype != t.dtype or old.device != t.device
+                    or old.is_inference() != t.is_inference()):  # fmt: skip
+                self.register_buffer(name, t, persistent=False)
+            else:  # what a captured graph reads stays where it is
+                old.copy_(t)
+        self._int8_marks = marks
         return self
+
+    def _weight_marks(self):
+        """Each expert weight with where it hangs and its version counter (None: torch keeps none for it). One
+        that is computed from other parameters does not hang there and is not watched."""
+        if self.expert_type == "swiglu":
+            hangs = [(self.experts._parameters, name) for name in ("w_gate_up", "w_down")]
+        else:
+            hangs = [(expert[i]._parameters, "weight") for expert in self.experts for i in (0, 2)]
+        found = [(d, name, d[name]) for d, name in hangs if d.get(name) is not None]
+        return [(d, name, w, None if w.is_inference() else w._version) for d, name, w in found]
 
     def dequantize(self):
         for name in ("w1_q", "w1_scale", "w2_q", "w2_scale"):
             if name in self._buffers:
                 del self._buffers[name]
+        self._int8_marks = None
         return self
 
     def _forward_int8(self, x, rows):
@@ -472,6 +492,10 @@ class MoEFeedForward(nn.Module):
         quantised, `rows`), and its int8 bytes and scale are what the dispatch copies top_k times."""
         if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
             raise ValueError("experts in int8 have no gradient: run them under torch.no_grad(), or dequantize() the layer")
+        if any(d.get(name) is not w or (v is not None and w._version != v) for d, name, w, v in self._int8_marks):
+            if torch.cuda.is_current_stream_capturing():  # the copies would only be filled by a replay
+                raise RuntimeError("the experts' weights changed since quantize_int8(): call it again before capturing")
+            self.quantize_int8()
         B, T, D = x.shape
         x_flat = x.reshape(-1, D)
         topk_w, topk_idx = routing.route_topk(self.router(x_flat), self.top_k, w_dtype=x.dtype)

@@ -306,3 +306,49 @@ def test_refusals():
     with pytest.raises(ValueError, match="scale must be float32"):
         routing.permute_int8_rows(rows._replace(scale=rows.scale[:3]), ix, 1)
     assert RMSNorm(8).weight.shape == (8,)
+
+
+@pytest.mark.parametrize("expert_type", ["swiglu", "gelu"])
+def test_a_layer_in_int8_follows_its_weights(expert_type):
+    """Weights that are loaded, written in place or replaced after quantize_int8() are the ones that run."""
+    import copy
+
+    torch.manual_seed(6)
+    kw = dict(expert_type=expert_type)
+    moe, other = (MoEFeedForward(64, 96, 4, 2, MoEImplementation.FAST, **kw).to(DEV) for _ in range(2))
+    x = torch.randn(2, 7, 64, device=DEV)
+    with torch.no_grad():
+        want = other.quantize_int8()(x)
+        moe.quantize_int8()
+        before = moe(x)
+        buffers = [moe.w1_q, moe.w1_scale, moe.w2_q, moe.w2_scale]
+        addresses = [t.data_ptr() for t in buffers]
+        moe.load_state_dict(other.state_dict())
+        assert torch.equal(moe(x), want) and not torch.equal(before, want)
+        # in place: what a captured graph reads stays where it is
+        assert [t.data_ptr() for t in (moe.w1_q, moe.w1_scale, moe.w2_q, moe.w2_scale)] == addresses
+        assert torch.equal(copy.deepcopy(moe)(x), want)
+        fresh = MoEFeedForward(64, 96, 4, 2, MoEImplementation.FAST, **kw).to(DEV)
+        fresh.router.weight.copy_(other.router.weight)
+        moe.load_state_dict({k: v.clone() for k, v in fresh.state_dict().items()}, assign=True)  # other Parameter objects
+        assert torch.equal(moe(x), fresh.quantize_int8()(x))
+        last = list(moe.experts.parameters())[-1]
+        last.mul_(2)  # the last (or the only) second weight
+        got = moe(x)
+        assert torch.equal(got, moe.quantize_int8()(x)) and not torch.equal(got, fresh(x))
+        # unseen by torch: the documented way is to quantise again, and a graph reads the refreshed copies
+        side = torch.cuda.Stream()
+        graph = torch.cuda.CUDAGraph()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(graph, stream=side):
+            captured = moe(x)
+        last.data.mul_(2)
+        want = moe.quantize_int8()(x)
+        graph.replay()
+        assert torch.equal(captured, want)
+        last.mul_(2)
+        with pytest.raises(RuntimeError, match="weights changed"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                moe(x)
+    torch.cuda.synchronize()
+    assert torch.isfinite(moe.dequantize()(x)).all()
