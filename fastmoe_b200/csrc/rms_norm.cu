@@ -822,6 +822,7 @@ static int launch_rows(const RowArgs& a, const RowShape& s, cudaStream_t st) {
 }
 
 constexpr int kBwdWarps = 8;  // rows per CTA where a warp takes a row
+constexpr int kBwdSmemMost = 220 * 1024;  // wider rows go through rms_bwd_loop_kernel
 
 // Shared memory of rms_bwd_kernel: the weight (where a warp takes a row the sum of the warps' dw) and the next row's slots.
 static int bwd_smem(const RowShape& s, int64_t D, int ve) {
@@ -835,11 +836,13 @@ static int launch_bwd(const RowBwdArgs& a, const RowShape& s, int grid, cudaStre
   const dim3 block = s.warp ? dim3(32, kBwdWarps) : dim3(s.threads);
   const int smem = bwd_smem(s, a.D, V);
   cudaError_t err = cudaSuccess;
+  // The attribute is one of the kernel, whoever launches it: every caller sets the same value, so that none lowers
+  // the limit between another thread's call here and its launch.
 #define FMOE_ROWS(CUT, VPT, WARP)                                                                                \
   do {                                                                                                           \
     if (smem > 40 * 1024) /* 48 KB is the limit for this and the static part together */                         \
       err = cudaFuncSetAttribute(rms_bwd_kernel<DT, CUT, VPT, WARP>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
-                                 smem);                                                                          \
+                                 kBwdSmemMost);                                                                  \
     if (err == cudaSuccess) rms_bwd_kernel<DT, CUT, VPT, WARP><<<grid, block, smem, st>>>(a);                     \
   } while (0)
   if (s.loop) rms_bwd_loop_kernel<DT><<<grid, 1024, 0, st>>>(a);
@@ -963,7 +966,7 @@ extern "C" int fmoe_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* 
   g.add(dx, D, T);
   g.weight(w);
   RowShape s = row_shape(g, D, T, dtype, true);
-  if (bwd_smem(s, D, g.ve) > 220 * 1024) s.loop = true;  // fp32 rows of more than 14000 columns
+  if (bwd_smem(s, D, g.ve) > kBwdSmemMost) s.loop = true;  // fp32 rows of more than 14000 columns
   const int grid = s.loop ? bwd_grid_most(T, D) : bwd_grid(T, s.threads, s.warp, s.vpt * (g.vec ? g.ve : 1));
   const RowBwdArgs a{dy, dsum, sum, rstd, w, dx, dw ? static_cast<float*>(scratch) : nullptr, T, D,
                      dy_stride, ds_stride, s_stride, 1.f / static_cast<float>(D), w_dtype == FMOE_F32, g.shift0, g.shift_step};

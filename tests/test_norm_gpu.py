@@ -358,3 +358,42 @@ def test_quantised_rows_are_exact():
             assert_quantised(rows.q, rows.scale, x)
             back = int8.dequantize_rows(rows, dtype)
             assert torch.equal(back, (rows.q.float() * rows.scale[:, None]).to(dtype))
+
+
+def test_backward_of_two_widths_from_two_threads():
+    """One instantiation serves rows of many widths with different amounts of shared memory; a call lets go of
+    the interpreter's lock, so two threads' calls interleave on the host."""
+    import threading
+
+    from fastmoe_b200 import _lib
+
+    T, calls, errors, outs = 300, 4000, [], {}
+    nbytes = {D: _lib.lib().fmoe_rms_norm_bwd_bytes(T, D) for D in (4104, 16384)}
+    data = {D: _inputs(T, D, torch.bfloat16) for D in nbytes}
+    torch.cuda.synchronize()
+
+    def work(D):
+        x, _, dy, _, w = data[D]
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            rstd = (1 / (x.double().square().mean(-1) + EPS).sqrt()).float()
+            dx, dw, scratch = torch.empty_like(x), torch.empty_like(w), torch.empty(nbytes[D], dtype=torch.uint8, device=DEV)
+        args = (dy.data_ptr(), D, None, 0, x.data_ptr(), D, rstd.data_ptr(), w.data_ptr(), _lib.FMOE_BF16, dx.data_ptr(),
+                dw.data_ptr(), scratch.data_ptr(), nbytes[D], T, D, _lib.FMOE_BF16, stream.cuda_stream)  # fmt: skip
+        try:
+            for _ in range(calls):
+                _lib.call("fmoe_rms_norm_bwd", *args)
+        except Exception as e:  # noqa: BLE001
+            errors.append((D, e))
+        stream.synchronize()
+        outs[D] = (dx, dw)
+
+    threads = [threading.Thread(target=work, args=(D,)) for D in nbytes]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for D, (dx, dw) in outs.items():
+        x, _, dy, _, w = data[D]
+        _check_backward(dx, dw, x, w, dy, None)
