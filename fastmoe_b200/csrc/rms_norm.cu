@@ -149,8 +149,19 @@ struct Vec<DT, kSingle> {
   __device__ __forceinline__ static uint32_t bits(uint32_t t) { return t; }
 };
 
+// Words that 16-bit weights e .. e + 7 lie in, from the word of e on: an odd e needs half of a fifth. The
+// vectors that are read so end before the last weight (e + 8 < D); no word of theirs reaches past it.
+__host__ __device__ constexpr int weight_words(int e) { return 4 + (e & 1); }
+constexpr bool weight_words_inside() {
+  for (int D = 9; D < 64; ++D)
+    for (int e = 1; e + 8 < D; ++e)
+      if ((e & ~1) + 2 * weight_words(e) > D) return false;
+  return true;
+}
+static_assert(weight_words_inside(), "a shifted row's weights are read inside the weight");
+
 // Weights e .. e + VE - 1, fp32 or of the rows' type, as floats; zeros outside the row. The weight
-// starts on the grid whatever the row does, so in a shifted row a vector of 16-bit weights comes in five words,
+// starts on the grid whatever the row does, so in a shifted row a vector of 16-bit weights comes in four or five words,
 // fp32 ones one by one, out of L1 (1714 x 7001 bf16: 17.2 us with single 16-bit ones, 15.5).
 template <int DT, int CUT>
 __device__ __forceinline__ void load_weight(const void* w, int w_f32, int e, int D, float* f) {
@@ -170,7 +181,7 @@ __device__ __forceinline__ void load_weight(const void* w, int w_f32, int e, int
     const uint32_t* from = reinterpret_cast<const uint32_t*>(static_cast<const E*>(w) + (e & ~1));
     uint32_t x[5];
 #pragma unroll
-    for (int i = 0; i < 5; ++i) x[i] = __ldg(from + i);
+    for (int i = 0; i < 5; ++i) x[i] = i < weight_words(e) ? __ldg(from + i) : 0u;
     if (e & 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] = __funnelshift_r(x[i], x[i + 1], 16);

@@ -397,3 +397,19 @@ def test_backward_of_two_widths_from_two_threads():
     for D, (dx, dw) in outs.items():
         x, _, dy, _, w = data[D]
         _check_backward(dx, dw, x, w, dy, None)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [11, 13, 15, 333, 1003, 7001, 8965])
+def test_nothing_behind_the_weight_counts(dtype, D):
+    """Every shift of rows of odd width, with NaN where the weight ends (what may be read is checked where the
+    kernels are compiled)."""
+    for T in (9, 400):
+        x, r, dy, ds, w = _inputs(T, D, dtype, seed=D)
+        behind = torch.full((D + 40,), float("nan"), dtype=dtype, device=DEV)
+        behind[:D] = w
+        xs, ws = x.clone().requires_grad_(True), behind[:D].requires_grad_(True)
+        y, s = norm.add_rms_norm(xs, r, ws, EPS)
+        _check_forward(y.detach(), s.detach(), w)
+        gx, gw = torch.autograd.grad((y, s), (xs, ws), (dy, ds))
+        _check_backward(gx, gw, s.detach(), w, dy, ds)
