@@ -207,27 +207,27 @@ class _PackedFFN(torch.autograd.Function):
     first weight's gradient) and the pre-activations; the hidden rows are recomputed from those."""
 
     @staticmethod
-    def forward(ctx, x, w1, w2, offsets, counts, act, row_map, covers_all_rows):
+    def forward(ctx, x, w1, w2, offsets, counts, act, row_map, covers_all_rows, origin):
         pre = torch.empty(x.shape[0], w1.shape[1], dtype=torch.bfloat16, device=x.device)
         hidden = _launch(x, w1, offsets, counts, act, covers_all_rows=covers_all_rows, pre=pre)
         out = _launch(hidden, w2, offsets, counts, ACT_NONE, row_map, covers_all_rows)
         p = checkpoint.pack_activation(pre)
         px = checkpoint.pack_activation(x) if ctx.needs_input_grad[1] else None
         ctx.save_for_backward(p.q, p.scale, None if px is None else px.q, None if px is None else px.scale, w1, w2,
-                              offsets, counts, row_map)  # fmt: skip
+                              offsets, counts, row_map, origin)  # fmt: skip
         ctx.shapes = (p.shape, x.shape)
         ctx.act, ctx.covers_all_rows = act, covers_all_rows
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
+        q, scale, xq, xscale, w1, w2, offsets, counts, row_map, origin = ctx.saved_tensors
         if torch.is_grad_enabled():  # create_graph
             with torch.no_grad():
                 grads = _PackedFFN.backward(ctx, grad_out)
             return tuple(None if g is None else
-                         ops._NoSecondDerivative.apply(g, "an FFN with packed activations", grad_out, *ctx.saved_tensors[4:6])
+                         ops._NoSecondDerivative.apply(g, "an FFN with packed activations", grad_out, w1, w2, origin)
                          for g in grads)  # fmt: skip
-        q, scale, xq, xscale, w1, w2, offsets, counts, row_map = ctx.saved_tensors
         pre_shape, x_shape = ctx.shapes
         if row_map is not None:
             grad_out = grad_out.index_select(0, row_map)  # back to the row order of `x`
@@ -246,7 +246,7 @@ class _PackedFFN(torch.autograd.Function):
             grad_w1 = _wgrad(grad_pre, x, w1.shape, offsets, counts)
         if ctx.needs_input_grad[0]:
             grad_x = _dgrad(grad_pre, w1, offsets, counts, ctx.covers_all_rows)
-        return grad_x, grad_w1, grad_w2, None, None, None, None, None
+        return grad_x, grad_w1, grad_w2, None, None, None, None, None, None
 
 
 def _packed_ffn(x, w1, w2, offsets, counts, act, row_map, covers_all_rows):
@@ -258,7 +258,9 @@ def _packed_ffn(x, w1, w2, offsets, counts, act, row_map, covers_all_rows):
         raise ValueError("row_map must be an int64 device tensor with one entry per row of x")
     check_shapes(w1.shape[1], w1.shape[2], act, True)
     check_shapes(w2.shape[1], w2.shape[2], ACT_NONE, True)
-    return _PackedFFN.apply(x.contiguous(), w1, w2, offsets, counts, act, row_map, covers_all_rows)
+    # x's place in the graph without its memory: what a gradient taken under create_graph is tied to
+    origin = x[:0].clone() if x.requires_grad else None
+    return _PackedFFN.apply(x.contiguous(), w1, w2, offsets, counts, act, row_map, covers_all_rows, origin)
 
 
 def _training(*tensors):

@@ -352,3 +352,32 @@ def test_a_layer_in_int8_follows_its_weights(expert_type):
                 moe(x)
     torch.cuda.synchronize()
     assert torch.isfinite(moe.dequantize()(x)).all()
+
+
+@pytest.mark.parametrize("act", ["swiglu", "gelu"])
+@pytest.mark.parametrize("free", ["x", "w1", "w2", "w1 w2", "x w1 w2"])
+def test_a_packed_ffn_with_frozen_parts_has_no_second_derivative(free, act):
+    """A penalty on a gradient is refused whatever requires one, not counted as a constant."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    t = dict(x=_randn(g, 9, 256), w1=_randn(g, 1, 512 if act == "swiglu" else 256, 256, scale=1 / 16),
+             w2=_randn(g, 1, 256, 256, scale=1 / 16))  # fmt: skip
+    leaves = [t[name].requires_grad_(True) for name in free.split()]
+    cnt = torch.tensor([9], device=DEV)
+    ffn = experts.grouped_swiglu_ffn if act == "swiglu" else experts.grouped_gelu_ffn
+    out = ffn(t["x"], t["w1"], t["w2"], cnt - cnt, cnt, covers_all_rows=True, packed=True)
+    plain = torch.autograd.grad(out.sum(), leaves, retain_graph=True)
+    grads = torch.autograd.grad(out.sum(), leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+    for gradient in grads:
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            # beside another loss, as a penalty is used
+            torch.autograd.grad(gradient.float().square().sum() + sum(p.float().sum() for p in leaves), leaves,
+                                retain_graph=True)  # fmt: skip
+    # accumulating them without a further derivative works
+    for p in leaves:
+        p.grad = None
+    out = ffn(t["x"], t["w1"], t["w2"], cnt - cnt, cnt, covers_all_rows=True, packed=True)
+    out.sum().backward(create_graph=True)
+    assert all(torch.equal(p.grad, a) for p, a in zip(leaves, plain))
+    for p in leaves:
+        p.grad = None
