@@ -41,6 +41,7 @@ def pack_activation(x: torch.Tensor) -> PackedActivation:
     _require_cuda(x, "x")
     if x.dim() < 1 or x.dtype not in _DTYPES or x.shape[-1] == 0:
         raise ValueError(f"x must be float32/bfloat16/float16 rows, got {tuple(x.shape)} {x.dtype}")
+    ops._refuse_tangents("pack_activation", x)
     x2 = _rows(x.detach())
     T, D = x2.shape
     Dp = _padded(D)
@@ -68,6 +69,7 @@ def _check_packed(p: PackedActivation):
 def unpack_activation(p: PackedActivation) -> torch.Tensor:
     """The values that `p` stands for, in the packed tensor's shape and type."""
     T, D = _check_packed(p)
+    ops._refuse_tangents("unpack_activation", p.scale)
     out = p.q.new_empty((T, D), dtype=p.dtype)
     ops._launch(p.q.get_device(), "fmoe_unpack_activation", 1, p.q.data_ptr(), p.q.stride(0), p.scale.data_ptr(),
                 out.data_ptr(), T, D, _DTYPES[p.dtype])  # fmt: skip
@@ -83,6 +85,7 @@ def _backward(p, grad, act):
     if grad.shape != want or grad.dtype != p.dtype or grad.device != p.q.device:
         raise ValueError(f"grad must be {want} {p.dtype} on {p.q.device}, got {tuple(grad.shape)} {grad.dtype} "
                          f"on {grad.device}")  # fmt: skip
+    ops._refuse_tangents("a derivative from packed activations", p.scale, grad)
     g2 = _rows(grad.detach())
     grad_h = g2.new_empty((T, D))
     hidden = g2.new_empty((T, cols))

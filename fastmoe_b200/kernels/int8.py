@@ -85,6 +85,7 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
         raise ValueError(f"x must be float32/bfloat16/float16 rows, got {tuple(x.shape)} {x.dtype}")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("quantize_rows has no gradient: call it under torch.no_grad() or on detached tensors")
+    ops._refuse_tangents("quantize_rows", x)
     x2 = _rows(x)
     T, K = x2.shape
     out = empty_rows(x2, T, K)
@@ -100,6 +101,7 @@ def dequantize_rows(rows: Int8Rows, dtype: torch.dtype = torch.bfloat16) -> torc
     _check_rows(q, scale)
     if dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {dtype}; use float32, bfloat16 or float16")
+    ops._refuse_tangents("dequantize_rows", scale)
     q, scale = _rows(q), scale.contiguous()
     T, K = q.shape
     out = q.new_empty((T, K), dtype=dtype)
@@ -113,6 +115,7 @@ def quantize_weight(w: torch.Tensor) -> Int8Weight:
     once per weight, not per call; a trained parameter is read through `w.detach()`."""
     if w.dim() not in (2, 3):
         raise ValueError(f"w must be [N, K] or [E, N, K], got {tuple(w.shape)}")
+    ops._refuse_tangents("quantize_weight", w)
     r = quantize_rows(w.detach())
     lead = w.shape[:-1]
     return Int8Weight(r.q.unflatten(0, lead) if w.dim() == 3 else r.q, r.scale.view(lead))
@@ -184,6 +187,7 @@ def _check_operands(a, w, dims, out_dtype):
         raise ValueError(f"K={K} could overflow the 32-bit sums (K <= {MAX_K})")
     if out_dtype not in _DTYPES:
         raise ValueError(f"unsupported out_dtype {out_dtype}; use float32, bfloat16 or float16")
+    ops._refuse_tangents("a product in 8 bits", a.scale, ws)
 
 
 def int8_linear(a: Int8Rows, w: Int8Weight, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:

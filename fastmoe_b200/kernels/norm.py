@@ -56,6 +56,7 @@ def _check(x, weight, residual, eps):
         )
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
+    ops._refuse_tangents("the RMS norm", x, weight, residual)
 
 
 def _empty(x):

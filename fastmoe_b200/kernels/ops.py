@@ -24,6 +24,7 @@ import os
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -313,6 +314,15 @@ def _launch(device: int, fn_name, n_kernels, *args):
         return _call(fn_name, n_kernels, *args, stream)
     launch_count += n_kernels
     return _lib.call(fn_name, *args, stream)
+
+
+def _refuse_tangents(what, *tensors):
+    """Raises where a tensor carries a forward-mode tangent: a kernel that runs beside autograd would return its
+    result without one, and that counts as a derivative of zero. Outside of forward mode this is one comparison."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 class _NoSecondDerivative(torch.autograd.Function):

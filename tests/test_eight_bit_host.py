@@ -104,3 +104,68 @@ def test_there_is_no_cpu_path():
     for call in calls:
         with pytest.raises(RuntimeError, match="no CPU path"):
             call()
+
+
+def _entry_points(x, w, q, scale):
+    """Every call of the three modules that takes floating-point tensors, by what it reads: (name, call)."""
+    rows, weight = int8.Int8Rows(q, scale), int8.Int8Weight(q, torch.ones(2))
+    packed = checkpoint.PackedActivation(q, torch.ones(2, 1), x.shape, x.dtype)
+    one = torch.zeros(1, dtype=torch.int64)
+    w3 = int8.Int8Weight(q[None], torch.ones(1, 2))
+    return [
+        ("x", lambda: norm.rms_norm(x, w)),
+        ("x", lambda: norm.add_rms_norm(x, torch.zeros(2, 16), w)),
+        ("x", lambda: norm.add_rms_norm(torch.zeros(2, 16), x, w)),
+        ("x", lambda: norm.rms_norm_int8(x, w)),
+        ("x", lambda: norm.rms_norm_int8(torch.zeros(2, 16), w, residual=x)),
+        ("x", lambda: int8.quantize_rows(x)),
+        ("x", lambda: int8.quantize_weight(x)),
+        ("x", lambda: checkpoint.pack_activation(x)),
+        ("x", lambda: checkpoint.packed_gelu_backward(packed, x)),
+        ("x", lambda: checkpoint.packed_swiglu_backward(packed, x[:, :8])),
+        ("w", lambda: norm.rms_norm(torch.zeros(2, 16), w)),
+        ("w", lambda: norm.rms_norm_int8(torch.zeros(2, 16), w)),
+        ("scale", lambda: int8.dequantize_rows(rows)),
+        ("scale", lambda: int8.int8_linear(rows, weight)),
+        ("scale", lambda: int8.int8_linear(int8.Int8Rows(q, torch.ones(2)), int8.Int8Weight(q, scale))),
+        ("scale", lambda: int8.grouped_int8_gemm(rows, w3, one, one)),
+        ("scale", lambda: int8.grouped_int8_gemm(int8.Int8Rows(q, torch.ones(2)), int8.Int8Weight(q[None], scale[None]), one, one)),
+        ("scale", lambda: checkpoint.unpack_activation(packed._replace(scale=scale[:, None]))),
+    ]
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The host's part of the calls without a device: CPU tensors pass, launches are counted and do nothing."""
+    from fastmoe_b200.kernels import ops
+
+    seen = []
+    for module in (norm, int8, checkpoint):
+        monkeypatch.setattr(module, "_require_cuda", lambda t, name: None)
+    monkeypatch.setattr(int8, "_status_word", lambda device: torch.zeros(1, dtype=torch.int32))
+    monkeypatch.setattr(ops, "_launch", lambda *args: seen.append(args[1]))
+    monkeypatch.setattr(ops, "_maybe_check", lambda *args: None)
+    return seen
+
+
+def test_forward_mode_is_refused_not_dropped(launches):
+    """A result without a tangent would count as one that does not depend on the input."""
+    from torch.autograd import forward_ad
+
+    given = dict(x=torch.randn(2, 16), w=torch.ones(16), q=torch.zeros(2, 16, dtype=torch.int8), scale=torch.ones(2))
+    n = len(_entry_points(**given))
+    for i in range(n):
+        _entry_points(**given)[i][1]()
+    assert len(launches) == n
+    with forward_ad.dual_level():
+        for i in range(n):  # nothing dual: they run
+            _entry_points(**given)[i][1]()
+        assert len(launches) == 2 * n
+        for i in range(n):
+            name = _entry_points(**given)[i][0]
+            dual = given | {name: forward_ad.make_dual(given[name], torch.ones_like(given[name]))}
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                _entry_points(**dual)[i][1]()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                _entry_points(**dual)[i][1]()
+        assert len(launches) == 2 * n
