@@ -37,10 +37,13 @@ class PackedActivation(NamedTuple):
 
 
 def pack_activation(x: torch.Tensor) -> PackedActivation:
-    """x (float32, bfloat16 or float16, any leading dimensions) in 8 bits."""
+    """x (float32, bfloat16 or float16, any leading dimensions) in 8 bits. No gradient flows through the packed
+    values: a leaf is read as it is, a tensor out of a graph is refused (pack `x.detach()`)."""
     _require_cuda(x, "x")
     if x.dim() < 1 or x.dtype not in _DTYPES or x.shape[-1] == 0:
         raise ValueError(f"x must be float32/bfloat16/float16 rows, got {tuple(x.shape)} {x.dtype}")
+    if x.requires_grad and not x.is_leaf and torch.is_grad_enabled():
+        raise ValueError("pack_activation has no gradient: call it under torch.no_grad() or on detached tensors")
     ops._refuse_tangents("pack_activation", x)
     x2 = _rows(x.detach())
     T, D = x2.shape
@@ -69,6 +72,8 @@ def _check_packed(p: PackedActivation):
 def unpack_activation(p: PackedActivation) -> torch.Tensor:
     """The values that `p` stands for, in the packed tensor's shape and type."""
     T, D = _check_packed(p)
+    if p.scale.requires_grad and torch.is_grad_enabled():
+        raise ValueError("unpack_activation has no gradient: call it under torch.no_grad() or on detached scales")
     ops._refuse_tangents("unpack_activation", p.scale)
     out = p.q.new_empty((T, D), dtype=p.dtype)
     ops._launch(p.q.get_device(), "fmoe_unpack_activation", 1, p.q.data_ptr(), p.q.stride(0), p.scale.data_ptr(),
@@ -85,6 +90,9 @@ def _backward(p, grad, act):
     if grad.shape != want or grad.dtype != p.dtype or grad.device != p.q.device:
         raise ValueError(f"grad must be {want} {p.dtype} on {p.q.device}, got {tuple(grad.shape)} {grad.dtype} "
                          f"on {grad.device}")  # fmt: skip
+    if (grad.requires_grad or p.scale.requires_grad) and torch.is_grad_enabled():
+        raise ValueError("a derivative from packed activations has no gradient itself: call it under torch.no_grad() "
+                         "or on detached tensors")  # fmt: skip
     ops._refuse_tangents("a derivative from packed activations", p.scale, grad)
     g2 = _rows(grad.detach())
     grad_h = g2.new_empty((T, D))

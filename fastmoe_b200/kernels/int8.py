@@ -15,7 +15,8 @@ q = round(v * 127 / a), scale = a / 127 with a its largest magnitude (at least 2
 ties to even; a row that holds NaN or infinity has scale NaN.
 
 Rows of q lie at 16-byte steps: `Int8Rows.q` and `Int8Weight.q` are views of padded storage
-where K is not a multiple of 16. Nothing here has a gradient.
+where K is not a multiple of 16. Nothing here has a gradient: a call whose inputs ask for one is refused
+(`quantize_weight` reads a parameter as it is).
 """
 
 from __future__ import annotations
@@ -101,6 +102,8 @@ def dequantize_rows(rows: Int8Rows, dtype: torch.dtype = torch.bfloat16) -> torc
     _check_rows(q, scale)
     if dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {dtype}; use float32, bfloat16 or float16")
+    if scale.requires_grad and torch.is_grad_enabled():
+        raise ValueError("dequantize_rows has no gradient: call it under torch.no_grad() or on detached scales")
     ops._refuse_tangents("dequantize_rows", scale)
     q, scale = _rows(q), scale.contiguous()
     T, K = q.shape
@@ -187,6 +190,8 @@ def _check_operands(a, w, dims, out_dtype):
         raise ValueError(f"K={K} could overflow the 32-bit sums (K <= {MAX_K})")
     if out_dtype not in _DTYPES:
         raise ValueError(f"unsupported out_dtype {out_dtype}; use float32, bfloat16 or float16")
+    if (a.scale.requires_grad or ws.requires_grad) and torch.is_grad_enabled():
+        raise ValueError("a product in 8 bits has no gradient: call it under torch.no_grad() or on detached scales")
     ops._refuse_tangents("a product in 8 bits", a.scale, ws)
 
 

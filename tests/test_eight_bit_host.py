@@ -107,30 +107,32 @@ def test_there_is_no_cpu_path():
 
 
 def _entry_points(x, w, q, scale):
-    """Every call of the three modules that takes floating-point tensors, by what it reads: (name, call)."""
+    """Every call of the three modules that takes floating-point tensors: the one that it is about, the call, and
+    whether it follows gradients ("yes"), refuses them ("no") or reads a value on purpose ("reads")."""
     rows, weight = int8.Int8Rows(q, scale), int8.Int8Weight(q, torch.ones(2))
     packed = checkpoint.PackedActivation(q, torch.ones(2, 1), x.shape, x.dtype)
-    one = torch.zeros(1, dtype=torch.int64)
-    w3 = int8.Int8Weight(q[None], torch.ones(1, 2))
+    zero, one = torch.zeros(2, 16), torch.zeros(1, dtype=torch.int64)
+    unit = int8.Int8Rows(q, torch.ones(2))
     return [
-        ("x", lambda: norm.rms_norm(x, w)),
-        ("x", lambda: norm.add_rms_norm(x, torch.zeros(2, 16), w)),
-        ("x", lambda: norm.add_rms_norm(torch.zeros(2, 16), x, w)),
-        ("x", lambda: norm.rms_norm_int8(x, w)),
-        ("x", lambda: norm.rms_norm_int8(torch.zeros(2, 16), w, residual=x)),
-        ("x", lambda: int8.quantize_rows(x)),
-        ("x", lambda: int8.quantize_weight(x)),
-        ("x", lambda: checkpoint.pack_activation(x)),
-        ("x", lambda: checkpoint.packed_gelu_backward(packed, x)),
-        ("x", lambda: checkpoint.packed_swiglu_backward(packed, x[:, :8])),
-        ("w", lambda: norm.rms_norm(torch.zeros(2, 16), w)),
-        ("w", lambda: norm.rms_norm_int8(torch.zeros(2, 16), w)),
-        ("scale", lambda: int8.dequantize_rows(rows)),
-        ("scale", lambda: int8.int8_linear(rows, weight)),
-        ("scale", lambda: int8.int8_linear(int8.Int8Rows(q, torch.ones(2)), int8.Int8Weight(q, scale))),
-        ("scale", lambda: int8.grouped_int8_gemm(rows, w3, one, one)),
-        ("scale", lambda: int8.grouped_int8_gemm(int8.Int8Rows(q, torch.ones(2)), int8.Int8Weight(q[None], scale[None]), one, one)),
-        ("scale", lambda: checkpoint.unpack_activation(packed._replace(scale=scale[:, None]))),
+        ("x", lambda: norm.rms_norm(x, w), "yes"),
+        ("x", lambda: norm.add_rms_norm(x, zero, w), "yes"),
+        ("x", lambda: norm.add_rms_norm(zero, x, w), "yes"),
+        ("w", lambda: norm.rms_norm(zero, w), "yes"),
+        ("x", lambda: norm.rms_norm_int8(x, w), "no"),
+        ("x", lambda: norm.rms_norm_int8(zero, w, residual=x), "no"),
+        ("w", lambda: norm.rms_norm_int8(zero, w), "no"),
+        ("x", lambda: int8.quantize_rows(x), "no"),
+        ("x", lambda: int8.quantize_weight(x), "reads"),
+        ("scale", lambda: int8.dequantize_rows(rows), "no"),
+        ("scale", lambda: int8.int8_linear(rows, weight), "no"),
+        ("scale", lambda: int8.int8_linear(unit, int8.Int8Weight(q, scale)), "no"),
+        ("scale", lambda: int8.grouped_int8_gemm(rows, int8.Int8Weight(q[None], torch.ones(1, 2)), one, one), "no"),
+        ("scale", lambda: int8.grouped_int8_gemm(unit, int8.Int8Weight(q[None], scale[None]), one, one), "no"),
+        ("x", lambda: checkpoint.pack_activation(x), "no"),
+        ("scale", lambda: checkpoint.unpack_activation(packed._replace(scale=scale[:, None])), "no"),
+        ("x", lambda: checkpoint.packed_gelu_backward(packed, x), "no"),
+        ("x", lambda: checkpoint.packed_swiglu_backward(packed, x[:, :8]), "no"),
+        ("scale", lambda: checkpoint.packed_gelu_backward(packed._replace(scale=scale[:, None]), x), "no"),
     ]
 
 
@@ -148,18 +150,22 @@ def launches(monkeypatch):
     return seen
 
 
+def _given():
+    return dict(x=torch.randn(2, 16), w=torch.ones(16), q=torch.zeros(2, 16, dtype=torch.int8), scale=torch.ones(2))
+
+
 def test_forward_mode_is_refused_not_dropped(launches):
     """A result without a tangent would count as one that does not depend on the input."""
     from torch.autograd import forward_ad
 
-    given = dict(x=torch.randn(2, 16), w=torch.ones(16), q=torch.zeros(2, 16, dtype=torch.int8), scale=torch.ones(2))
+    given = _given()
     n = len(_entry_points(**given))
-    for i in range(n):
-        _entry_points(**given)[i][1]()
+    for _, call, _ in _entry_points(**given):
+        call()
     assert len(launches) == n
     with forward_ad.dual_level():
-        for i in range(n):  # nothing dual: they run
-            _entry_points(**given)[i][1]()
+        for _, call, _ in _entry_points(**given):  # nothing dual: they run
+            call()
         assert len(launches) == 2 * n
         for i in range(n):
             name = _entry_points(**given)[i][0]
@@ -169,3 +175,24 @@ def test_forward_mode_is_refused_not_dropped(launches):
             with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
                 _entry_points(**dual)[i][1]()
         assert len(launches) == 2 * n
+
+
+def test_a_gradient_is_refused_not_dropped(launches):
+    """What runs beside autograd and is given something out of a graph says so; under no_grad it runs."""
+    given = _given()
+    for i in range(len(_entry_points(**given))):
+        name = _entry_points(**given)[i][0]
+        out_of_a_graph = given | {name: given[name].clone().requires_grad_(True) * 1}
+        _, call, follows = _entry_points(**out_of_a_graph)[i]
+        with torch.no_grad():
+            call()
+        launches.clear()
+        if follows == "no":
+            with pytest.raises(ValueError, match="no gradient"):
+                call()
+            assert not launches
+        else:
+            result = call()
+            result = result[0] if isinstance(result, tuple) else result
+            assert len(launches) == 1 and result.requires_grad == (follows == "yes")
+    checkpoint.pack_activation(torch.randn(2, 16).requires_grad_(True))  # a leaf is read as it is
