@@ -336,6 +336,19 @@ class MoEFeedForward(nn.Module):
         return torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16
 
     def _use_grouped(self, recv_data):
+        if self._grouped_serves(recv_data):
+            return True
+        if self.pack_activations and torch.is_grad_enabled() and (
+            recv_data.requires_grad or any(p.requires_grad for p in self.experts.parameters())
+        ):
+            raise ValueError(
+                "pack_activations: these experts do not run grouped, so their activations would be kept unpacked; it needs "
+                f"bfloat16 rows on a CUDA device{' (or bfloat16 autocast)' if self.expert_type == 'gelu' else ''} and widths "
+                f"that the grouped product tiles, got {recv_data.dtype} rows of {self.dim} on {recv_data.device}"
+            )
+        return False
+
+    def _grouped_serves(self, recv_data):
         if self.implementation != consts.MoEImplementation.FAST or not recv_data.is_cuda:
             return False
         if self.expert_type == "swiglu":

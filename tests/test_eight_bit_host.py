@@ -196,3 +196,22 @@ def test_a_gradient_is_refused_not_dropped(launches):
             result = result[0] if isinstance(result, tuple) else result
             assert len(launches) == 1 and result.requires_grad == (follows == "yes")
     checkpoint.pack_activation(torch.randn(2, 16).requires_grad_(True))  # a leaf is read as it is
+
+
+@pytest.mark.parametrize("expert_type", ["gelu", "swiglu"])
+def test_packing_that_is_not_served_is_refused(expert_type):
+    """Where the experts would train with their activations unpacked all the same; without gradients nothing is
+    kept, and they run."""
+    from fastmoe_b200.consts import MoEImplementation
+    from fastmoe_b200.models.tiny_model import MoEFeedForward
+
+    moe = MoEFeedForward(64, 32, 2, 1, MoEImplementation.FAST, expert_type=expert_type, pack_activations=True)
+    x = torch.randn(6, 64)
+    with pytest.raises(ValueError, match="pack_activations"):
+        moe.compute_experts(x, [2, 4])
+    with torch.no_grad():
+        assert moe.compute_experts(x, [2, 4]).shape == (6, 64)
+    moe.requires_grad_(False)
+    assert moe.compute_experts(x, [2, 4]).shape == (6, 64)
+    with pytest.raises(ValueError, match="pack_activations"):
+        moe.compute_experts(x.requires_grad_(True), [2, 4])

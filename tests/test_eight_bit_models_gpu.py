@@ -381,3 +381,22 @@ def test_a_packed_ffn_with_frozen_parts_has_no_second_derivative(free, act):
     assert all(torch.equal(p.grad, a) for p, a in zip(leaves, plain))
     for p in leaves:
         p.grad = None
+
+
+def test_packing_is_refused_where_it_has_no_effect():
+    x = torch.randn(2, 9, 256, device=DEV)
+    kw = dict(pack_activations=True)
+    for moe, rows in ((MoEFeedForward(256, 256, 4, 2, MoEImplementation.FAST, expert_type="swiglu", **kw).to(DEV), x),
+                      (MoEFeedForward(256, 256, 4, 2, MoEImplementation.FAST, **kw).to(DEV), x),
+                      # 200 columns are no size of the grouped product
+                      (MoEFeedForward(200, 256, 4, 2, MoEImplementation.FAST, **kw).to(DEV).to(BF16), x[..., :200].to(BF16))):
+        with pytest.raises(ValueError, match="pack_activations"):
+            moe(rows)
+        with torch.no_grad():
+            assert torch.isfinite(moe(rows)).all()
+    # fp32 GELU modules under autocast are served
+    moe = MoEFeedForward(256, 256, 4, 2, MoEImplementation.FAST, **kw).to(DEV)
+    with torch.autocast("cuda", BF16):
+        out = moe(x)
+    out.float().square().sum().backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in moe.experts.parameters())
