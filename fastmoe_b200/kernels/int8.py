@@ -161,9 +161,11 @@ def _product(a, w, offsets, counts, act, out, E):
     N, K = wshape[-2:]
     R = aq.shape[0]
     dev = aq.get_device()
+    # a single row (or expert) may have any stride
+    w_row = wstride[-2] if N > 1 else _padded(K)
     ops._launch(
         dev, "fmoe_int8_gemm", 1, aq.data_ptr(), aq.stride(0) if R > 1 else _padded(K), sa.data_ptr(), wq.data_ptr(),
-        wstride[-2], wstride[0] if len(wshape) == 3 else 0, sw.data_ptr(), out.data_ptr(),
+        w_row, wstride[0] if E > 1 else N * w_row, sw.data_ptr(), out.data_ptr(),
         None if offsets is None else offsets.data_ptr(), None if counts is None else counts.data_ptr(), E, R, N, K, act,
         _DTYPES[out.dtype], _status_word(aq.device).data_ptr(),
     )  # fmt: skip

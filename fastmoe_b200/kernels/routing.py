@@ -165,7 +165,7 @@ def permute_int8_rows(rows: Int8Rows, ix: RoutingIndex, K: int) -> Int8Rows:
     _check_rows(rows.q, rows.scale)
     q = _operand(rows.q)
     T, D = q.shape
-    if D % 16:  # the rows travel with their padding, as 16-bit words
-        q = q.as_strided((T, _padded(D)), (q.stride(0), 1))
+    if D % 16 or T == 1:  # the rows travel with their padding, as 16-bit words; a single row may have any stride
+        q = q.as_strided((T, _padded(D)), (q.stride(0) if T > 1 else _padded(D), 1))
     words = permute_rows(q.view(torch.bfloat16), ix.slot_of, K)
     return Int8Rows(words.view(torch.int8)[:, :D], rows.scale[ix.reverse_map])

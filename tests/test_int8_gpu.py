@@ -373,3 +373,38 @@ def test_waits_that_run_out_are_reported(kernel):
         _lib.tune("gemm_spin_limit", 1 << 24)
     _check(int8.int8_linear(a, w), _product64(a, w.q, w.scale), "none", torch.bfloat16)
     assert ops.read_status() == 0 and experts.ACT_NONE == 0
+
+
+def test_a_single_row_has_any_stride():
+    """One output channel, one expert or one token, cut out of something wider: its stride says nothing."""
+    K = 64
+    a, w = _case(5, K, 3, 4, seed=1)  # three experts of four channels
+    wide = torch.full((4, K + 9), 5, dtype=torch.int8, device=DEV)
+    wide[0, :K] = w.q[0, 0]
+    one = wide[:1, :K]
+    assert one.is_contiguous() and one.stride(0) == K + 9
+    narrow = torch.empty(K, 1, dtype=torch.int8, device=DEV)
+    narrow[:, 0] = w.q[0, 0]
+    off, cnt = _spread([5])
+    for q in (one, narrow.t()):
+        out = int8.int8_linear(a, Int8Weight(q, w.scale[0, :1]), out_dtype=torch.float32)
+        _check(out, _product64(a, q, w.scale[0, :1]), "none", torch.float32)
+        out = int8.grouped_int8_gemm(a, Int8Weight(q[None], w.scale[:1, :1]), off, cnt, out_dtype=torch.float32)
+        _check(out, _product64(a, q, w.scale[0, :1]), "none", torch.float32)
+    expert = torch.empty(4 * K + 7, dtype=torch.int8, device=DEV).as_strided((1, 4, K), (4 * K + 7, K, 1))
+    expert.copy_(w.q[:1])
+    out = int8.grouped_int8_gemm(a, Int8Weight(expert, w.scale[:1]), off, cnt, out_dtype=torch.float32)
+    _check(out, _product64(a, w.q[0], w.scale[0]), "none", torch.float32)
+    # one token
+    token = Int8Rows(one, a.scale[:1])
+    out = int8.int8_linear(token, Int8Weight(w.q[1], w.scale[1]), out_dtype=torch.float32)
+    _check(out, _product64(token, w.q[1], w.scale[1]), "none", torch.float32)
+    from fastmoe_b200.kernels import routing
+
+    ix = routing.build_index(torch.tensor([[1, 0]], device=DEV), torch.ones(1, 2, device=DEV), 3)
+    for q, size in ((one, K), (narrow.t(), K), (wide[:1, : K - 3], K - 3)):
+        rows = routing.permute_int8_rows(Int8Rows(q, a.scale[:1]), ix, 2)
+        assert torch.equal(rows.q, q.expand(2, size)) and torch.equal(rows.scale, a.scale[:1].expand(2))
+    assert torch.equal(int8.dequantize_rows(token, torch.float32), one.float() * a.scale[0])
+    torch.cuda.synchronize()
+    assert ops.read_status() == 0
