@@ -413,3 +413,25 @@ def test_nothing_behind_the_weight_counts(dtype, D):
         _check_forward(y.detach(), s.detach(), w)
         gx, gw = torch.autograd.grad((y, s), (xs, ws), (dy, ds))
         _check_backward(gx, gw, s.detach(), w, dy, ds)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [2, 300])
+def test_every_width_is_right(T, dtype):
+    """Block shapes and shared memory go by the width: a step of 61 columns passes through all of them, and
+    the widths around their borders follow. Each output of each of them is looked at."""
+    borders = [k * v + d for v in (4, 8) for k in (32, 64, 128, 256, 512, 1024, 2048) for d in (-1, 0, 1, v - 1)]
+    for D in sorted({*range(61, 9000, 61), *borders}):
+        x, r, dy, ds, w = _inputs(T, D, dtype, seed=D)
+        x.requires_grad_(True)
+        w.requires_grad_(True)
+        y, s = norm.add_rms_norm(x, r, w, EPS)
+        gx, gw = torch.autograd.grad((y, s), (x, w), (dy, ds))
+        s, w = s.detach(), w.detach()
+        _check_forward(y.detach(), s, w)
+        _check_backward(gx, gw, s, w, dy, ds)
+        out = norm.rms_norm_int8(x.detach(), w, EPS, residual=r, with_y=True)
+        assert torch.equal(out.stream, s) and torch.equal(out.y, y)
+        _assert_norm_quantised(out.rows, s, w)
+        rows = int8.quantize_rows(s)
+        assert_quantised(rows.q, rows.scale, s)
