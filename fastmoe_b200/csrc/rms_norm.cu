@@ -8,9 +8,10 @@
 //
 // Every kernel is bound by HBM: a row is read once, held in registers across its reductions, and
 // every output is written once. The sum of squares runs in 64 bits: the 8-bit output rounds next
-// to borders, and with a 64-bit sum the fp32 result does not depend on how the row is split over
-// threads, so a row quantises the same in a batch of one and in a batch of thousands. It costs
-// one conversion and one fused multiply-add per element, far below what a row's bytes take.
+// to borders. How a row is split over threads then moves rstd in fp32 only where it lies within some 2^-50 of
+// a border between two fp32 values, so a row quantises the same in a batch of one and in a batch of
+// thousands, but for about one row in 2^25. It costs one conversion and one fused multiply-add per
+// element, far below what a row's bytes take.
 #include "int8.cuh"
 
 namespace fmoe {
@@ -833,7 +834,9 @@ static int launch_rows(const RowArgs& a, const RowShape& s, cudaStream_t st) {
 }
 
 constexpr int kBwdWarps = 8;  // rows per CTA where a warp takes a row
-constexpr int kBwdSmemMost = 220 * 1024;  // wider rows go through rms_bwd_loop_kernel
+// Wider rows go through rms_bwd_loop_kernel, three to four times as slow: fp32 3584 x 16384 385 us, floor 108 (bf16
+// 7168 x 16384, the same bytes, 145).
+constexpr int kBwdSmemMost = 220 * 1024;
 
 // Shared memory of rms_bwd_kernel: the weight (where a warp takes a row the sum of the warps' dw) and the next row's slots.
 static int bwd_smem(const RowShape& s, int64_t D, int ve) {
@@ -977,7 +980,7 @@ extern "C" int fmoe_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* 
   g.add(dx, D, T);
   g.weight(w);
   RowShape s = row_shape(g, D, T, dtype, true);
-  if (bwd_smem(s, D, g.ve) > kBwdSmemMost) s.loop = true;  // fp32 rows of more than 14000 columns
+  if (bwd_smem(s, D, g.ve) > kBwdSmemMost) s.loop = true;  // fp32 rows of more than 13312 columns
   const int grid = s.loop ? bwd_grid_most(T, D) : bwd_grid(T, s.threads, s.warp, s.vpt * (g.vec ? g.ve : 1));
   const RowBwdArgs a{dy, dsum, sum, rstd, w, dx, dw ? static_cast<float*>(scratch) : nullptr, T, D,
                      dy_stride, ds_stride, s_stride, 1.f / static_cast<float>(D), w_dtype == FMOE_F32, g.shift0, g.shift_step};

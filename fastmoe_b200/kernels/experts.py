@@ -271,7 +271,8 @@ def grouped_swiglu_ffn(x, w_gate_up, w_down, offsets, counts, row_map=None, cove
     """down(silu(gate(x)) * up(x)) per expert. w_gate_up [E, 2*ff, D] (gate rows first), w_down [E, D, ff].
     `row_map` reorders the rows of the result (see grouped_gemm). `packed=True`: a forward that will
     be differentiated keeps the rows and the pre-activations in 8 bits and no hidden rows
-    (`kernels/checkpoint.py`): the result is the same, the gradients are taken at the kept values."""
+    (`kernels/checkpoint.py`): the result is the same, the gradients are taken at the kept values. Their
+    own derivative is refused."""
     if packed and _training(x, w_gate_up, w_down):
         return _packed_ffn(x, w_gate_up, w_down, offsets, counts, ACT_SWIGLU, row_map, bool(covers_all_rows))
     hidden = grouped_gemm(x, w_gate_up, offsets, counts, activation=ACT_SWIGLU, covers_all_rows=covers_all_rows)

@@ -9,7 +9,8 @@
 The norm of a pre-norm block (`models/tiny_model.py`, `norm="rms"`); the reference's blocks
 normalise with LayerNorm (src/fastmoe/models/tiny_model.py:424-463). Rows are the last dimension,
 in float32, bfloat16 or float16; the weight is float32 or of the rows' type. Statistics, products
-and gradients are computed in 32 bits or more and rounded once.
+and gradients are computed in 32 bits or more and rounded once. There is a gradient, no second derivative
+and no forward mode: both are refused.
 """
 
 from __future__ import annotations
