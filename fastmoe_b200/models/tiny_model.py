@@ -29,6 +29,8 @@ There is no CPU path: inputs must live on a CUDA device.
 
 from __future__ import annotations
 
+import weakref
+
 import torch
 import torch.distributed as dist
 import torch.nn as nn
@@ -96,6 +98,37 @@ class Int8Linear(nn.Module):
             rows = int8.quantize_rows(x)
         out = int8.int8_linear(rows, int8.Int8Weight(self.weight_q, self.weight_scale), out_dtype=x.dtype)
         return out.view(*x.shape[:-1], out.shape[-1])
+
+
+class _WeightWatch:
+    """Which weights 8-bit copies were made of, and their version counters. They are held weakly: moving or dropping
+    the floating-point weights frees them. A copy of a watch (deepcopy, pickle) has seen none yet."""
+
+    def __init__(self, owners=None):
+        """`owners`: (module, name of its parameter). A weight that is computed from other parameters is not
+        watched; version None: torch does not count the writes."""
+        self.seen = None if owners is None else [
+            (weakref.ref(m), name, weakref.ref(w), None if w.is_inference() else w._version)
+            for m, name, w in ((m, name, m._parameters.get(name)) for m, name in owners) if w is not None
+        ]  # fmt: skip
+
+    def __reduce__(self):
+        return _WeightWatch, ()
+
+    def changed(self, device, owners):
+        """Whether one of the weights, of those that are on `device`, is another one or has been written since.
+        `owners()` gives the weights of today."""
+        if self.seen is None:
+            weights = [m._parameters.get(name) for m, name in owners()]
+            return bool(weights) and all(w is None or w.device == device for w in weights)
+        for module, name, weight, version in self.seen:
+            owner = module()
+            w = None if owner is None else owner._parameters.get(name)
+            if w is None or (w is weight() and (version is None or w._version == version)):
+                continue
+            if w.device == device:
+                return True
+        return False
 
 
 class MultiheadSelfAttention(nn.Module):
@@ -462,12 +495,12 @@ class MoEFeedForward(nn.Module):
         """From now on `forward` runs the experts in 8-bit integers (kernels/int8.py), for inference: the
         weights are quantised here, once, with a scale per output channel. The router stays as it is.
         The floating-point weights are kept; `dequantize()` returns to them. Where they have been written or
-        replaced since (`load_state_dict`, an update in place), the next `forward` quantises them again. A
-        write that torch does not count (through `.data`), and a captured graph, need this call again: it
-        refreshes the 8-bit weights in place. Single rank only."""
+        replaced since (`load_state_dict`, an update in place), the next `forward` quantises them again, unless
+        they have left the device. A write that torch does not count (through `.data`), other expert modules,
+        and a captured graph need this call again: it refreshes the 8-bit weights in place. Single rank only."""
         if self.world_size > 1 or getattr(self, "_fused_exchange", None) is not None:
             raise ValueError("experts in int8 run on a single rank: rows do not travel in 8 bits")
-        marks = self._weight_marks()
+        watch = _WeightWatch(self._weight_owners())
         if self.expert_type == "swiglu":
             w1, w2 = int8.quantize_weight(self.experts.w_gate_up), int8.quantize_weight(self.experts.w_down)
         else:
@@ -480,24 +513,23 @@ class MoEFeedForward(nn.Module):
                 self.register_buffer(name, t, persistent=False)
             else:  # what a captured graph reads stays where it is
                 old.copy_(t)
-        self._int8_marks = marks
+        self._int8_watch = watch
         return self
 
-    def _weight_marks(self):
-        """Each expert weight with where it hangs and its version counter (None: torch keeps none for it). One
-        that is computed from other parameters does not hang there and is not watched."""
+    def _weight_owners(self):
+        """(module, name of its parameter) of each expert weight; none where the experts have been dropped."""
+        experts = getattr(self, "experts", None)
+        if experts is None:
+            return []
         if self.expert_type == "swiglu":
-            hangs = [(self.experts._parameters, name) for name in ("w_gate_up", "w_down")]
-        else:
-            hangs = [(expert[i]._parameters, "weight") for expert in self.experts for i in (0, 2)]
-        found = [(d, name, d[name]) for d, name in hangs if d.get(name) is not None]
-        return [(d, name, w, None if w.is_inference() else w._version) for d, name, w in found]
+            return [(experts, "w_gate_up"), (experts, "w_down")]
+        return [(expert[i], "weight") for expert in experts for i in (0, 2)]
 
     def dequantize(self):
         for name in ("w1_q", "w1_scale", "w2_q", "w2_scale"):
             if name in self._buffers:
                 del self._buffers[name]
-        self._int8_marks = None
+        self._int8_watch = None
         return self
 
     def _forward_int8(self, x, rows):
@@ -505,7 +537,7 @@ class MoEFeedForward(nn.Module):
         quantised, `rows`), and its int8 bytes and scale are what the dispatch copies top_k times."""
         if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
             raise ValueError("experts in int8 have no gradient: run them under torch.no_grad(), or dequantize() the layer")
-        if any(d.get(name) is not w or (v is not None and w._version != v) for d, name, w, v in self._int8_marks):
+        if self._int8_watch.changed(self.w1_q.device, self._weight_owners):
             if torch.cuda.is_current_stream_capturing():  # the copies would only be filled by a replay
                 raise RuntimeError("the experts' weights changed since quantize_int8(): call it again before capturing")
             self.quantize_int8()

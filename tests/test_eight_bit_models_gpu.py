@@ -400,3 +400,34 @@ def test_packing_is_refused_where_it_has_no_effect():
         out = moe(x)
     out.float().square().sum().backward()
     assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in moe.experts.parameters())
+
+
+@pytest.mark.parametrize("expert_type", ["swiglu", "gelu"])
+def test_a_layer_in_int8_without_its_floating_point_weights(expert_type, tmp_path):
+    """It runs on its 8-bit copies: the weights may be moved off the device or dropped, which frees them, and the
+    layer may be copied and saved."""
+    import copy
+
+    torch.manual_seed(7)
+    moe = MoEFeedForward(512, 1024, 8, 2, MoEImplementation.FAST, expert_type=expert_type).to(DEV)
+    x = torch.randn(2, 7, 512, device=DEV)
+    with torch.no_grad():
+        want = moe.quantize_int8()(x)
+        torch.save(moe, tmp_path / "moe.pt")
+        loaded = torch.load(tmp_path / "moe.pt", weights_only=False)
+        assert torch.equal(loaded(x), want) and torch.equal(copy.deepcopy(moe)(x), want)
+        size = sum(p.numel() * p.element_size() for p in moe.experts.parameters())
+        del loaded
+        before = torch.cuda.memory_allocated()
+        moe.experts.to("cpu")
+        assert torch.equal(moe(x), want)
+        assert torch.cuda.memory_allocated() <= before - size
+        assert torch.equal(copy.deepcopy(moe)(x), want)
+        for p in moe.experts.parameters():
+            p.mul_(2)
+        assert torch.equal(moe(x), want)  # not there to be read
+        moe.experts.to(DEV)
+        got = moe(x)
+        assert torch.equal(got, moe.quantize_int8()(x)) and not torch.equal(got, want)
+        moe.experts = None
+        assert torch.equal(moe(x), got) and torch.equal(copy.deepcopy(moe)(x), got)
